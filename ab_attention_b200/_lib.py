@@ -48,6 +48,9 @@ _SIGNATURES = {
     "abx_sparse_prefill_scatter": ([_p, _p, _p, _i64, _i64, _p, _p, _i64, _p, _p, _i64, _p, ctypes.c_int, _i64,
                                     _i64, _p, _p, ctypes.c_size_t, _p], ctypes.c_int),
     "abx_dense_prefill": ([_p, _p, _p, _i64, _i64, _p, _p, _p], ctypes.c_int),
+    "abx_rotary": ([_p, _p], ctypes.c_int),
+    "abx_chunk_workspace_size": ([_p, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "abx_chunk_attention": ([_p, _p, ctypes.c_size_t, _p], ctypes.c_int),
     "abx_cross_prefill": ([_p, _i64, _p, _p, _i64, _i64, _p, _p, _i64, _p, _p, _i64, _p, _p, _p], ctypes.c_int),
 }
 

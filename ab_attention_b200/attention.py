@@ -193,3 +193,24 @@ def dense_cross_attention(q, k, v, *, extra_kv=None, return_lse=False):
                                  text_k=tk, text_v=tv, return_lse=return_lse)
     out = out.reshape_as(q)
     return (out, lse.reshape(batch, heads, tokens)) if return_lse else out
+
+
+@torch.no_grad()
+def window_attention(q, k, v, *, window=None, sinks=0, block=1, return_lse=False):
+    """Causal attention (scale 128^-0.5) with a sliding window and sinks over contiguous keys.
+
+    q [B,H,N,128], k and v [B,Hk,Nk,128] with Hk dividing H; bf16 or fp16; any N and Nk. The
+    queries are the last N of the Nk positions: query i sits at p = Nk - N + i and sees key j
+    when ``j < e`` and (``j >= e - window`` or ``j < sinks``), ``e = (p // block + 1) * block``.
+    block 1 is causal; with a larger block (a video frame's tokens) every token sees to the
+    end of its block, and ``window`` counts back from there. window=None: no limit. A
+    row that sees nothing gives zeros and an lse of -inf. Single tokens (N = 1) against a
+    long k take the same call. Tiles that no query sees are not read. ``return_lse`` adds the
+    base-2 LSE [B,H,N]. `chunk_attention` is the form over a paged cache.
+    """
+    if q.device.type == "cpu":
+        raise ValueError("B200 attention requires CUDA tensors")
+    if window is not None and window < 1:
+        raise ValueError("window must be positive, or None")
+    out, lse = torch.ops.ab_attention.window_attention(q, k, v, window or 0, sinks, block)
+    return (out, lse) if return_lse else out

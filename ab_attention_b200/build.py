@@ -23,8 +23,9 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libabx.so"
 TORCH_LIB = PKG / "libabx_torch.so"  # torch.ops.ab_attention (csrc/torch_ops.cpp)
-SOURCES = ("ibcs.cu", "sip.cu", "prefill.cu", "prefill_pair.cu", "capi.cu")
-HEADERS = ("common.cuh", "ibcs.cuh", "tcgen05.cuh", "tma_host.cuh", "f32x2.cuh", "mix.cuh")
+SOURCES = ("ibcs.cu", "sip.cu", "prefill.cu", "prefill_pair.cu", "rotary.cu", "chunk_token.cu",
+           "capi.cu")
+HEADERS = ("common.cuh", "ibcs.cuh", "tcgen05.cuh", "tma_host.cuh", "f32x2.cuh", "mix.cuh", "rotary.cuh", "chunk.cuh")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-lineinfo", "--use_fast_math", "-Xcompiler", "-fPIC",
@@ -83,14 +84,17 @@ def build_torch_ops(force: bool, run) -> Path:
     from torch.utils import cpp_extension
 
     src = CSRC / "torch_ops.cpp"
-    if not (force or _stale(TORCH_LIB, [src, LIB, ROOT / "include" / "abx.h"])):
+    if not (force or _stale(TORCH_LIB, [src, LIB, Path(__file__), ROOT / "include" / "abx.h"])):
         return TORCH_LIB
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     includes = [f"-I{p}" for p in [str(ROOT / "include"), *cpp_extension.include_paths("cuda")]]
     libdirs = cpp_extension.library_paths("cuda")
+    # libstdc++ by its shared object: a compiler that would link its archive instead leaves a second
+    # copy of the iostream code beside torch's, and an error message that prints sizes ends the process.
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            *includes, str(src), "-o", str(TORCH_LIB), f"-L{PKG}", "-l:libabx.so",
            *[f"-L{d}" for d in libdirs], "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+           "-l:libstdc++.so.6",
            "-Wl,-rpath,$ORIGIN", *[f"-Wl,-rpath,{d}" for d in libdirs]]
     run(cmd)
     return TORCH_LIB

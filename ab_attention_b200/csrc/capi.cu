@@ -5,14 +5,18 @@
 // synchronisation (except abx_device_status, which reads the error word).
 #include <cuda.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
 
+#include "chunk.cuh"
 #include "common.cuh"
 #include "ibcs.cuh"
+#include "rotary.cuh"
 #include "tcgen05.cuh"
+#include "tma_host.cuh"
 
 namespace abx {
 
@@ -639,6 +643,234 @@ int abx_selftest_wait_timeout(int64_t limit_cycles, abx_stream_t stream) {
         return fail(ABX_ERR_INVALID_ARGUMENT, "limit must be in (0, 4e9] cycles");
     abx::wait_selftest_kernel<<<1, 64, 0, stream>>>(static_cast<uint64_t>(limit_cycles), abx::device_error_word());
     return check_cuda(cudaGetLastError(), "self-test launch");
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Streaming operators: rotary positions, cache append, chunk attention.
+// ---------------------------------------------------------------------------
+namespace {
+
+// Every row (batch, head, token) of a [.., 128] tensor starts on a 16-byte boundary.
+int check_rows(const char* name, const void* p, const int64_t (&stride)[3], int element_bytes) {
+    if (p == nullptr) return fail(ABX_ERR_INVALID_ARGUMENT, "%s must be non-null", name);
+    if (!aligned16(p)) return fail(ABX_ERR_INVALID_ARGUMENT, "%s must be 16-byte aligned", name);
+    for (int64_t s : stride)
+        if (s < 0 || s * element_bytes % 16 != 0)
+            return fail(ABX_ERR_INVALID_ARGUMENT, "the strides of %s must be multiples of 16 bytes (got %lld elements)",
+                        name, (long long)s);
+    return ABX_OK;
+}
+
+int check_pages(int64_t sequences, int64_t table_width, int64_t page_size, int64_t pages) {
+    if (sequences < 1 || sequences > 0x3fffffff) return fail(ABX_ERR_INVALID_ARGUMENT, "there must be at least one sequence");
+    if (page_size < 16 || (page_size < 128 ? (page_size & (page_size - 1)) != 0 : page_size % 128 != 0))
+        return fail(ABX_ERR_INVALID_ARGUMENT, "page size must be 16, 32, 64 or a multiple of 128 (got %lld)", (long long)page_size);
+    if (pages < 1 || pages > 0x3fffffff) return fail(ABX_ERR_INVALID_ARGUMENT, "the cache must have pages (got %lld)", (long long)pages);
+    if (table_width < 1) return fail(ABX_ERR_INVALID_ARGUMENT, "the page table must have columns");
+    if (page_size > abx::kMaxCacheKeys || table_width > abx::kMaxCacheKeys / page_size)
+        return fail(ABX_ERR_UNSUPPORTED, "more than 2^30 cache positions a sequence");
+    return ABX_OK;
+}
+
+// [128, tokens, heads, pages] with 64-column x box_rows boxes (128-byte swizzle). A
+// dim of one element may have any stride; the map wants one that it can encode.
+cudaError_t encode_cache(CUtensorMap* map, const void* base, bool fp16, int64_t tokens, int64_t heads, int64_t pages,
+                         const int64_t (&stride)[3], uint32_t box_rows) {
+    auto encode = abx::tensor_map_encoder();
+    if (encode == nullptr) return cudaErrorNotSupported;
+    const cuuint64_t dims[4] = {abx::kHeadDim, static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(heads),
+                                static_cast<cuuint64_t>(pages)};
+    const int64_t step[3] = {tokens > 1 ? stride[2] : abx::kHeadDim, heads > 1 ? stride[1] : abx::kHeadDim,
+                             pages > 1 ? stride[0] : abx::kHeadDim};
+    const cuuint64_t bytes[3] = {static_cast<cuuint64_t>(step[0]) * 2, static_cast<cuuint64_t>(step[1]) * 2,
+                                 static_cast<cuuint64_t>(step[2]) * 2};
+    const cuuint32_t box[4] = {64, box_rows, 1, 1};
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                              const_cast<void*>(base), dims, bytes, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+int64_t at_most(int64_t x, int64_t most) { return x < most ? x : most; }
+
+// Checks every argument of a chunk call that does not need the device, and lays the call out.
+int chunk_plan(const abx_chunk_args* c, abx::ChunkArgs& a, size_t& workspace) {
+    if (c == nullptr) return fail(ABX_ERR_INVALID_ARGUMENT, "args is null");
+    if (c->dtype != ABX_BF16 && c->dtype != ABX_FP16) return fail(ABX_ERR_INVALID_ARGUMENT, "attention takes bf16 or fp16");
+    const bool paged = c->page_table != nullptr;
+    if (c->sequences < 1 || c->tokens < 1) return fail(ABX_ERR_INVALID_ARGUMENT, "there must be sequences and tokens");
+    if (c->kv_heads < 1 || c->kv_heads > 65535 || c->heads < 1 || c->heads % c->kv_heads != 0)
+        return fail(ABX_ERR_INVALID_ARGUMENT, "heads (%lld) must be a multiple of kv_heads (%lld)", (long long)c->heads,
+                    (long long)c->kv_heads);
+    if (c->window < 0 || c->sinks < 0 || c->block < 1)
+        return fail(ABX_ERR_INVALID_ARGUMENT, "window and sinks must not be negative, block must be positive");
+    if (int st = check_rows("q", c->q, c->q_stride, 2)) return st;
+    if (int st = check_rows("k", c->k, c->k_stride, 2)) return st;
+    if (int st = check_rows("v", c->v, c->v_stride, 2)) return st;
+    if (int st = check_rows("o", c->o, c->o_stride, 2)) return st;
+    if (c->longest < 1 || c->longest > c->tokens)
+        return fail(ABX_ERR_INVALID_ARGUMENT, "longest must be in [1, tokens] (got %lld)", (long long)c->longest);
+    if (paged) {
+        if (int st = check_pages(c->sequences, c->table_width, c->page_size, c->pages)) return st;
+        if (c->starts == nullptr || c->lengths == nullptr)
+            return fail(ABX_ERR_INVALID_ARGUMENT, "starts and lengths must be non-null");
+    } else {
+        if (c->keys < 1) return fail(ABX_ERR_INVALID_ARGUMENT, "there must be keys");
+        if (c->keys > abx::kMaxCacheKeys || c->sequences > 0x3fffffff) return fail(ABX_ERR_UNSUPPORTED, "more than 2^30 keys");
+        if (c->longest != c->tokens) return fail(ABX_ERR_INVALID_ARGUMENT, "longest must be the token count");
+    }
+    const int64_t all_tokens = paged ? c->tokens : c->tokens * c->sequences;
+    if (c->heads > 0x3fffffff || c->tokens > 0x3fffffff / c->heads || all_tokens > 0x7fffffff)
+        return fail(ABX_ERR_UNSUPPORTED, "too many query rows");
+    const int64_t largest = 0x3fffffff;
+    a = abx::ChunkArgs{};
+    a.q = c->q;
+    a.o = c->o;
+    a.lse = c->lse;
+    a.q_seq = paged ? 0 : c->q_stride[0], a.q_head = c->q_stride[1], a.q_token = c->q_stride[2];
+    a.o_seq = paged ? 0 : c->o_stride[0], a.o_head = c->o_stride[1], a.o_token = c->o_stride[2];
+    a.l_seq = paged ? 0 : c->lse_stride[0], a.l_head = c->lse_stride[1], a.l_token = c->lse_stride[2];
+    a.starts = paged ? c->starts : nullptr;
+    a.lengths = paged ? c->lengths : nullptr;
+    a.table = c->page_table;
+    a.seqs = static_cast<int32_t>(c->sequences);
+    a.heads = static_cast<int32_t>(c->heads);
+    a.kv_heads = static_cast<int32_t>(c->kv_heads);
+    a.group = static_cast<int32_t>(c->heads / c->kv_heads);
+    a.tokens = static_cast<int32_t>(c->tokens);
+    a.longest = static_cast<int32_t>(c->longest);
+    a.keys = static_cast<int32_t>(paged ? c->table_width * c->page_size : c->keys);
+    a.table_width = static_cast<int32_t>(paged ? c->table_width : 0);
+    a.page_size = static_cast<int32_t>(paged ? c->page_size : 0);
+    a.pages = static_cast<int32_t>(paged ? c->pages : c->sequences);
+    a.window = c->window == 0 ? abx::kNoWindow : static_cast<int32_t>(at_most(c->window, largest));
+    a.sinks = c->window == 0 ? 0 : static_cast<int32_t>(at_most(c->sinks, largest));
+    a.block = static_cast<int32_t>(at_most(c->block, largest));
+    a.rows_total = all_tokens * c->heads;
+    a.kappa = abx::qk_scale_log2();
+    abx::chunk_layout(a);
+    workspace = a.splits > 1 ? align_up(static_cast<size_t>(a.splits) * a.rows_total * abx::kHeadDim * 4) +
+                                   align_up(static_cast<size_t>(a.splits) * a.rows_total * 4)
+                             : 0;
+    return ABX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int abx_rotary(const abx_rotary_args* r, abx_stream_t stream) {
+    if (r == nullptr) return fail(ABX_ERR_INVALID_ARGUMENT, "args is null");
+    const bool paged = r->page_table != nullptr;
+    if (r->dtype != ABX_BF16 && r->dtype != ABX_FP16 && (paged || r->dtype != ABX_F32))
+        return fail(ABX_ERR_INVALID_ARGUMENT, "rotary takes bf16, fp16 or (without a cache) f32");
+    const int e = r->dtype == ABX_F32 ? 4 : 2;
+    if (r->batch < 1 || r->tokens < 1 || (paged && r->batch != 1))
+        return fail(ABX_ERR_INVALID_ARGUMENT, "there must be tokens (one batch of them with a page table)");
+    if (r->tokens > 0x7fffffff / r->batch) return fail(ABX_ERR_UNSUPPORTED, "too many tokens");
+    if (r->heads < 0 || r->kv_heads < 0 || r->heads > 0xffffff || r->kv_heads > 0xffffff)
+        return fail(ABX_ERR_INVALID_ARGUMENT, "bad head count");
+    const bool has_q = r->q != nullptr, has_k = r->k != nullptr;
+    if ((!has_q && !has_k) || (has_q && r->heads < 1) || (has_k && r->kv_heads < 1) || (paged && !has_k))
+        return fail(ABX_ERR_INVALID_ARGUMENT, "q or k (with a page table, k and v) must be given with their heads");
+    if (has_q || !paged) {
+        if (r->positions == nullptr) return fail(ABX_ERR_INVALID_ARGUMENT, "positions must be non-null");
+    }
+    abx::RotaryArgs a{};
+    if (r->positions != nullptr) {
+        if (r->axes < 1 || r->axes > abx::kRotaryAxes)
+            return fail(ABX_ERR_INVALID_ARGUMENT, "between 1 and %d axes (got %d)", abx::kRotaryAxes, r->axes);
+        if (!(r->theta > 0) || !std::isfinite(r->theta)) return fail(ABX_ERR_INVALID_ARGUMENT, "theta must be positive");
+        int dims = 0;
+        for (int x = 0; x < r->axes; ++x) {
+            if (r->sections[x] < 0 || r->sections[x] > abx::kHeadDim || r->sections[x] % 2 != 0)
+                return fail(ABX_ERR_INVALID_ARGUMENT, "sections must be even");
+            dims += r->sections[x];
+        }
+        if (dims != abx::kHeadDim) return fail(ABX_ERR_INVALID_ARGUMENT, "sections must sum to 128 (got %d)", dims);
+        int pair = 0;
+        for (int x = 0; x < r->axes; ++x)
+            for (int i = 0; i < r->sections[x] / 2; ++i, ++pair) {
+                const double power = r->shared ? 2.0 * pair / abx::kHeadDim : 2.0 * i / r->sections[x];
+                a.freq[pair] = std::pow(r->theta, -power) / 3.14159265358979323846;
+                a.axis[pair] = static_cast<uint8_t>(x);
+            }
+    }
+    auto add = [&](const char* name, const void* src, const int64_t (&s)[3], void* dst, const int64_t (&d)[3],
+                   int64_t heads, bool turn, bool to_cache) -> int {
+        if (int st = check_rows(name, src, s, e)) return st;
+        if (int st = check_rows("the output", dst, d, e)) return st;
+        abx::RotaryJob& j = a.job[a.jobs++];
+        j = abx::RotaryJob{src, dst, s[0], s[1], s[2], d[0], d[1], d[2], static_cast<int32_t>(heads), turn, to_cache};
+        a.heads += j.heads;
+        return ABX_OK;
+    };
+    if (has_q)
+        if (int st = add("q", r->q, r->q_stride, r->q_out, r->q_out_stride, r->heads, true, false)) return st;
+    if (has_k)
+        if (int st = add("k", r->k, r->k_stride, r->k_out, r->k_out_stride, r->kv_heads, r->positions != nullptr, paged))
+            return st;
+    if (paged) {
+        if (int st = add("v", r->v, r->v_stride, r->v_out, r->v_out_stride, r->kv_heads, false, true)) return st;
+        if (int st = check_pages(r->sequences, r->table_width, r->page_size, r->pages)) return st;
+        if (r->starts == nullptr || r->lengths == nullptr)
+            return fail(ABX_ERR_INVALID_ARGUMENT, "starts and lengths must be non-null");
+        a.starts = r->starts;
+        a.lengths = r->lengths;
+        a.table = r->page_table;
+        a.seqs = static_cast<int32_t>(r->sequences);
+        a.table_width = static_cast<int32_t>(r->table_width);
+        a.page_size = static_cast<int32_t>(r->page_size);
+        a.pages = static_cast<int32_t>(r->pages);
+    }
+    a.positions = r->positions;
+    a.p_batch = r->positions_batch;
+    a.axes = r->axes;
+    a.batch = static_cast<int32_t>(r->batch);
+    a.tokens = static_cast<int32_t>(r->tokens);
+    a.halves = r->halves != 0;
+    a.sign = r->inverse ? -1.f : 1.f;
+    a.error = abx::device_error_word();
+    return check_cuda(abx::launch_rotary(a, r->dtype, stream), "rotary launch");
+}
+
+int abx_chunk_workspace_size(const abx_chunk_args* args, size_t* bytes) {
+    if (bytes == nullptr) return fail(ABX_ERR_INVALID_ARGUMENT, "bytes is null");
+    abx::ChunkArgs a;
+    return chunk_plan(args, a, *bytes);
+}
+
+int abx_chunk_attention(const abx_chunk_args* args, void* workspace, size_t workspace_bytes, abx_stream_t stream) {
+    abx::ChunkArgs a;
+    size_t need = 0;
+    if (int st = chunk_plan(args, a, need)) return st;
+    if (need > 0) {
+        if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % kAlign != 0)
+            return fail(ABX_ERR_WORKSPACE, "workspace must be non-null and 256-byte aligned");
+        if (workspace_bytes < need)
+            return fail(ABX_ERR_WORKSPACE, "workspace too small (%zu < %zu bytes)", workspace_bytes, need);
+        a.part_o = static_cast<float*>(workspace);
+        a.part_lse = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                              align_up(static_cast<size_t>(a.splits) * a.rows_total * abx::kHeadDim * 4));
+    }
+    a.error = abx::device_error_word();
+    const bool fp16 = args->dtype == ABX_FP16;
+    const int tile_keys = abx::chunk_tile_keys(a);
+    const int box_rows = a.table == nullptr || a.page_size > tile_keys ? tile_keys : a.page_size;
+    const int64_t tokens = a.table == nullptr ? a.keys : a.page_size;
+    abx::ChunkMaps maps;
+    if (int st = check_cuda(encode_cache(&maps.k, args->k, fp16, tokens, a.kv_heads, a.pages, args->k_stride, box_rows),
+                            "tensor map of k"))
+        return st;
+    if (int st = check_cuda(encode_cache(&maps.v, args->v, fp16, tokens, a.kv_heads, a.pages, args->v_stride, box_rows),
+                            "tensor map of v"))
+        return st;
+    if (int st = check_cuda(abx::launch_chunk(a, maps, fp16, box_rows, stream), "chunk attention launch")) return st;
+    return a.splits > 1 ? check_cuda(abx::launch_chunk_join(a, fp16, stream), "chunk join launch") : ABX_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,219 @@
+// Attention of new tokens over a key/value cache: what its kernels share.
+//
+// Query token i of a sequence with n new tokens and `len` keys (the new ones
+// included) sits at position p = len - n + i and sees key j when
+//     j < min(e, len)  and  (j >= e - window  or  j < sinks),   e = (p / block + 1) * block
+// (block 1: causal; a larger block sees to its own end). Query heads share key
+// heads in groups of G, and the (token, head) pairs of a group are the rows of
+// one problem: row r is token r / G, head kvh * G + r % G. The keys a tile of
+// rows needs are walked in tiles; a tile that no row sees is not read.
+//
+// The keys lie in pages ([pages, kv_heads, page_size, 128] with a page table)
+// or, without a table, in one "page" a sequence ([B, kv_heads, keys, 128]).
+#pragma once
+
+#include <cuda.h>
+
+#include "common.cuh"
+
+namespace abx {
+
+struct ChunkArgs {
+    const void* q;
+    void* o;
+    float* lse;            // nullptr: not written
+    int64_t q_seq, q_head, q_token;  // strides in elements; q_seq is 0 when tokens are packed
+    int64_t o_seq, o_head, o_token;
+    int64_t l_seq, l_head, l_token;
+    float* part_o;         // [splits, rows_total, 128] f32, normalised by the split's own sum
+    float* part_lse;       // [splits, rows_total] base 2; -inf: the split saw nothing
+    const int32_t* starts;   // [seqs + 1] or nullptr (every sequence has `tokens` tokens)
+    const int32_t* lengths;  // [seqs] or nullptr (every sequence has `keys` keys)
+    const int32_t* table;    // [seqs, table_width] or nullptr (sequence s is page s)
+    int32_t seqs, heads, kv_heads, group;
+    int32_t tokens;        // per sequence, or, packed, of all sequences
+    int32_t longest;       // tokens of the longest sequence
+    int32_t keys;          // per sequence, or, paged, at most (table_width * page_size)
+    int32_t table_width, page_size, pages;
+    int32_t window, sinks, block;  // window: kNoWindow without one
+    int32_t splits;        // CTAs that share the keys of one row tile
+    int32_t span;          // key tiles of one split, or 0: the row tile's keys in equal parts
+    int64_t rows_total;    // tokens of all sequences * heads
+    float kappa;           // 128^-0.5 * log2(e)
+    int* error;
+};
+
+constexpr int32_t kNoWindow = 0x40000000;
+constexpr int32_t kMaxCacheKeys = 0x3fffffff;
+
+// One tile of rows of one sequence.
+struct ChunkUnit {
+    int32_t seq;    // -1: none (past the last tile)
+    int32_t row0;   // first row
+    int32_t n;      // the sequence's new tokens
+    int32_t len;    // its keys
+    int32_t first;  // its first token in the packed arrays (0 when not packed)
+};
+
+// Tokens [a, b) and key count of packed sequence s, clipped to what the buffers hold.
+__device__ __forceinline__ void chunk_sequence(const ChunkArgs& a, int s, int32_t& first, int32_t& n, int32_t& len,
+                                               bool& bad) {
+    const int32_t s0 = __ldg(a.starts + s), s1 = __ldg(a.starts + s + 1), l = __ldg(a.lengths + s);
+    first = min(max(s0, 0), a.tokens);
+    const int32_t last = min(max(s1, first), a.tokens);
+    n = last - first;
+    len = min(max(l, 0), a.keys);
+    bad = s0 != first || s1 != last || l != len || n > a.longest;
+    if (n > a.longest) n = 0;  // more tokens than the launch covers: reported and not computed
+}
+
+// The row tile that unit u of the grid works on; called by whole warps. Tiles of
+// a sequence come last first: under a causal mask the longest rows start first.
+__device__ __forceinline__ ChunkUnit chunk_unit(const ChunkArgs& a, int u, int tile_rows) {
+    ChunkUnit r{-1, 0, 0, 0, 0};
+    if (a.starts == nullptr) {
+        const int tiles = (a.tokens * a.group + tile_rows - 1) / tile_rows;
+        r.seq = u / tiles;
+        r.row0 = (tiles - 1 - (u - r.seq * tiles)) * tile_rows;
+        r.n = a.tokens;
+        r.len = a.keys;
+        return r;
+    }
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int base = 0; base < a.seqs; base += 32) {
+        const int s = base + lane;
+        int32_t first = 0, n = 0, len = 0, tiles = 0;
+        if (s < a.seqs) {
+            bool bad;
+            chunk_sequence(a, s, first, n, len, bad);
+            if (bad) raise_device_error(a.error, ABX_ERR_INVALID_ARGUMENT);
+            tiles = static_cast<int32_t>((static_cast<int64_t>(n) * a.group + tile_rows - 1) / tile_rows);
+        }
+        int sum = tiles;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int other = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += other;
+        }
+        const unsigned reached = __ballot_sync(0xffffffffu, before + sum > u);
+        if (reached) {
+            const int at = __ffs(reached) - 1;
+            const int tiles_before = before + __shfl_sync(0xffffffffu, sum - tiles, at);
+            tiles = __shfl_sync(0xffffffffu, tiles, at);
+            r.seq = base + at;
+            r.row0 = (tiles - 1 - (u - tiles_before)) * tile_rows;
+            r.n = __shfl_sync(0xffffffffu, n, at);
+            r.len = __shfl_sync(0xffffffffu, len, at);
+            r.first = __shfl_sync(0xffffffffu, first, at);
+            return r;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return r;
+}
+
+// Keys [0, sink) and [low, end) are what a query sees.
+struct Seen {
+    int32_t sink, low, end;
+};
+
+__device__ __forceinline__ Seen chunk_seen(const ChunkArgs& a, const ChunkUnit& u, int row) {
+    const int32_t p = u.len - u.n + row / a.group;
+    const int32_t e = p < 0 ? 0 : (a.block == 1 ? p + 1 : (p / a.block + 1) * a.block);
+    Seen s;
+    s.end = min(e, u.len);
+    s.low = min(max(e - a.window, 0), s.end);
+    s.sink = min(a.sinks, s.low);
+    return s;
+}
+
+// The key tiles of rows [row0, row1]: [0, head) then [low, low + count - head).
+struct KeyTiles {
+    int32_t head, low, count;
+    Seen first, last;  // of the first and the last row: every bound grows with the row
+    __device__ __forceinline__ int32_t tile(int i) const { return i < head ? i : low + (i - head); }
+    // Whether any row of the tile sees key j.
+    __device__ __forceinline__ bool any(int32_t j) const {
+        return j < last.end && (j >= first.low || j < last.sink);
+    }
+};
+
+template <int kKeys>
+__device__ __forceinline__ KeyTiles chunk_tiles(const ChunkArgs& a, const ChunkUnit& u, int row0, int row1) {
+    KeyTiles t;
+    t.first = chunk_seen(a, u, row0);
+    t.last = chunk_seen(a, u, row1);
+    const int32_t high = (t.last.end + kKeys - 1) / kKeys;
+    t.low = min(t.first.low / kKeys, high);
+    t.head = min((t.last.sink + kKeys - 1) / kKeys, t.low);
+    t.count = t.head + high - t.low;
+    return t;
+}
+
+// The part [begin, end) of `count` key tiles that split `s` takes.
+__device__ __forceinline__ void chunk_part(const ChunkArgs& a, int count, int s, int& begin, int& end) {
+    if (a.span > 0) {
+        begin = min(s * a.span, count);
+        end = min(begin + a.span, count);
+    } else {
+        begin = static_cast<int>(static_cast<int64_t>(count) * s / a.splits);
+        end = static_cast<int>(static_cast<int64_t>(count) * (s + 1) / a.splits);
+    }
+}
+
+// Page of the `box` keys from j on for the K/V tensor maps: `pages` (which reads
+// zeros) where no row sees any of them (their page may be long gone) or the table names no page.
+__device__ __forceinline__ int32_t chunk_page(const ChunkArgs& a, const ChunkUnit& u, const KeyTiles& t, int32_t j,
+                                              int32_t box) {
+    if (a.table == nullptr) return u.seq;
+    if (j >= t.last.end || (j + box <= t.first.low && j >= t.last.sink)) return a.pages;
+    const int32_t page = __ldg(a.table + static_cast<int64_t>(u.seq) * a.table_width + j / a.page_size);
+    if (page < 0 || page >= a.pages) {
+        raise_device_error(a.error, ABX_ERR_INVALID_ARGUMENT);
+        return a.pages;
+    }
+    return page;
+}
+
+// Of K and V: [128, tokens of a page, kv_heads, pages], 64 columns x `rows` tokens a box, 128-byte swizzle.
+struct ChunkMaps {
+    CUtensorMap k, v;
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int32_t x, int32_t y, int32_t z, int32_t w,
+                                            uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+
+// 16-bit pairs of the two element types.
+template <class T>
+struct Pair;
+template <>
+struct Pair<bf16> {
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&p);
+    }
+};
+template <>
+struct Pair<half> {
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        __half2 p = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&p);
+    }
+};
+
+// Chooses the splits of a call (and, by its sizes, the kernel that launch_chunk takes).
+void chunk_layout(ChunkArgs& args);
+int chunk_tile_keys(const ChunkArgs& args);
+
+// The launchers. Arguments are validated by the C ABI layer.
+cudaError_t launch_chunk(const ChunkArgs& args, const ChunkMaps& maps, bool fp16, int box_rows, cudaStream_t stream);
+cudaError_t launch_chunk_join(const ChunkArgs& args, bool fp16, cudaStream_t stream);
+
+}  // namespace abx

@@ -223,6 +223,87 @@ int abx_cross_prefill(const void* q, int64_t q_tokens, const void* k, const void
                       const int32_t* ids, const float* log_weights, int64_t samples, const void* text_k,
                       const void* text_v, int64_t text_tokens, void* o, float* lse, abx_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Streaming operators (no counterpart in the reference): rotary positions, a paged
+ * key/value cache, and attention of new tokens over it. Element types: bf16 or
+ * fp16 (rotary without a cache also f32); head dim 128. Strides are in elements,
+ * the innermost dim is contiguous, and every row starts on a 16-byte boundary.
+ * ------------------------------------------------------------------------- */
+enum abx_dtype { ABX_BF16 = 0, ABX_FP16 = 1, ABX_F32 = 2 };
+
+/* Rotary positions over up to four axes. Axis a turns sections[a] of the head's
+ * 128 dims (even; they sum to 128), in order. Pair i of an axis with d dims turns
+ * by position * theta^(-2i / d), or, shared, pair i of the whole head (of its 64)
+ * by position * theta^(-2i / 128). Pairs are dims (2i, 2i + 1), or, halves,
+ * (i, i + 64). inverse turns back, which is also the turn's gradient. Angles are
+ * taken in 64 bits.
+ *
+ * q, k, v are rows (batch, head, token); q_out and k_out get the turned rows. Any
+ * of the three may be NULL (with its heads 0). positions: int32 [batch or 1,
+ * tokens, axes]. v is only used with a page table.
+ *
+ * With page_table the call appends to a cache: batch is 1, tokens are packed
+ * (sequence s owns tokens [starts[s], starts[s + 1]), and its last token goes to
+ * cache position lengths[s] - 1), and k_out / v_out are the cache, strides (page,
+ * head, token of a page), both [pages, kv_heads, page_size, 128]. positions may be
+ * NULL: k is stored as it is (and q must be NULL). A token outside every
+ * sequence is not stored; one whose place is outside the table, or whose table
+ * entry names no page, is not stored and records ABX_ERR_INVALID_ARGUMENT in the
+ * device error word. Two tokens with one place leave either's row. */
+typedef struct abx_rotary_args {
+  int32_t dtype;
+  int32_t axes;
+  int32_t sections[4];
+  double theta;
+  int32_t shared, halves, inverse;
+  const int32_t* positions;
+  int64_t positions_batch; /* stride of positions between batches, 0: one for all */
+  int64_t batch, tokens;
+  const void *q, *k, *v;
+  void *q_out, *k_out, *v_out;
+  int64_t heads, kv_heads;
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* batch, head, token */
+  int64_t q_out_stride[3], k_out_stride[3], v_out_stride[3];
+  const int32_t *starts, *lengths, *page_table; /* [sequences + 1], [sequences], [sequences, table_width] */
+  int64_t sequences, table_width, page_size, pages;
+} abx_rotary_args;
+int abx_rotary(const abx_rotary_args* args, abx_stream_t stream);
+
+/* Attention (scale 128^-0.5) of new tokens over the keys so far, those of the new
+ * tokens included. Token i of a sequence with n new tokens and `len` keys is at
+ * position p = len - n + i and sees key j when j < min(e, len) and (j >= e - window
+ * or j < sinks), e = (p / block + 1) * block, none for p < 0: causal for block 1; a
+ * block of tokens otherwise sees to its own end. window 0: no limit. A row that
+ * sees nothing gives zeros and an lse of -inf. heads is a multiple of kv_heads; head
+ * h reads key head h / (heads / kv_heads).
+ *
+ * Contiguous (page_table NULL): q and o rows (sequence, head, token) of `tokens`
+ * tokens a sequence, k and v rows (sequence, head, token) of `keys` tokens.
+ * Paged: tokens are packed (`tokens` of all sequences; starts / lengths as above; the
+ * sequence strides of q, o and lse are ignored), k and v are rows (page, head, token
+ * of a page). page_size is 16, 32, 64 or a multiple of 128. longest bounds the tokens
+ * of any sequence; a sequence with more is not computed and records
+ * ABX_ERR_INVALID_ARGUMENT, as do lengths or starts past the buffers (clipped)
+ * and table entries that name no page (read as zeros). Rows of tokens in no
+ * sequence are left as they were. The cached rows of a sequence have to be
+ * finite; what lies behind them in its last page may be anything.
+ *   lse f32 rows (sequence, head, token), base 2; NULL to skip.
+ * The workspace (device memory, 256-byte aligned) joins keys that several CTAs
+ * share; abx_chunk_workspace_size may report 0. */
+typedef struct abx_chunk_args {
+  int32_t dtype;
+  const void *q, *k, *v;
+  void* o;
+  float* lse;
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3], lse_stride[3];
+  int64_t sequences, tokens, longest, keys, heads, kv_heads;
+  const int32_t *starts, *lengths, *page_table;
+  int64_t table_width, page_size, pages;
+  int64_t window, sinks, block;
+} abx_chunk_args;
+int abx_chunk_workspace_size(const abx_chunk_args* args, size_t* bytes);
+int abx_chunk_attention(const abx_chunk_args* args, void* workspace, size_t workspace_bytes, abx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
