@@ -23,8 +23,8 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libabx.so"
 TORCH_LIB = PKG / "libabx_torch.so"  # torch.ops.ab_attention (csrc/torch_ops.cpp)
-SOURCES = ("ibcs.cu", "sip.cu", "prefill.cu", "prefill_pair.cu", "rotary.cu", "chunk_token.cu",
-           "capi.cu")
+SOURCES = ("ibcs.cu", "sip.cu", "prefill.cu", "prefill_pair.cu", "rotary.cu", "chunk.cu", "chunk_token.cu",
+           "chunk_tile.cu", "capi.cu")
 HEADERS = ("common.cuh", "ibcs.cuh", "tcgen05.cuh", "tma_host.cuh", "f32x2.cuh", "mix.cuh", "rotary.cuh", "chunk.cuh")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [

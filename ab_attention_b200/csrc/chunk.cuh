@@ -14,6 +14,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace abx {
@@ -36,6 +38,7 @@ struct ChunkArgs {
     int32_t keys;          // per sequence, or, paged, at most (table_width * page_size)
     int32_t table_width, page_size, pages;
     int32_t window, sinks, block;  // window: kNoWindow without one
+    int32_t tile_rows;     // rows of a tile: 16 or 32 (chunk_token.cu), 256 (chunk_tile.cu)
     int32_t splits;        // CTAs that share the keys of one row tile
     int32_t span;          // key tiles of one split, or 0: the row tile's keys in equal parts
     int64_t rows_total;    // tokens of all sequences * heads
@@ -45,6 +48,8 @@ struct ChunkArgs {
 
 constexpr int32_t kNoWindow = 0x40000000;
 constexpr int32_t kMaxCacheKeys = 0x3fffffff;
+constexpr int kChunkTokenKeys = 64;  // keys of a tile of each kernel
+constexpr int kChunkTileKeys = 128;
 
 // One tile of rows of one sequence.
 struct ChunkUnit {
@@ -208,12 +213,15 @@ struct Pair<half> {
     }
 };
 
-// Chooses the splits of a call (and, by its sizes, the kernel that launch_chunk takes).
+// Chooses the kernel (tile_rows) and the splits of a call.
 void chunk_layout(ChunkArgs& args);
+int64_t chunk_units(const ChunkArgs& args);  // row tiles of a key head, at most
 int chunk_tile_keys(const ChunkArgs& args);
 
 // The launchers. Arguments are validated by the C ABI layer.
 cudaError_t launch_chunk(const ChunkArgs& args, const ChunkMaps& maps, bool fp16, int box_rows, cudaStream_t stream);
+cudaError_t launch_chunk_token(const ChunkArgs& args, const ChunkMaps& maps, bool fp16, int box_rows, cudaStream_t stream);
+cudaError_t launch_chunk_tile(const ChunkArgs& args, const ChunkMaps& maps, bool fp16, int box_rows, cudaStream_t stream);
 cudaError_t launch_chunk_join(const ChunkArgs& args, bool fp16, cudaStream_t stream);
 
 }  // namespace abx

@@ -17,7 +17,7 @@
 namespace abx {
 namespace {
 
-constexpr int kKeys = 64;                       // keys of a tile
+constexpr int kKeys = kChunkTokenKeys;          // keys of a tile
 constexpr int kWarpKeys = 16;
 constexpr int kWarps = kKeys / kWarpKeys;       // consumers
 constexpr int kThreads = (kWarps + 1) * 32;     // and the loader
@@ -331,56 +331,13 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
     if (tid == 0 && *abort_flag) raise_device_error(a.error, ABX_ERR_DEVICE_TIMEOUT);
 }
 
-// Joins the splits of each row: o = sum_s 2^(lse_s - lse) o_s. One warp a row, four dims a lane;
-// reads splits * 516 bytes a row.
-template <class T>
-__global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= a.rows_total) return;
-    const int64_t token = row / a.heads;
-    const int head = static_cast<int>(row - token * a.heads);
-    int64_t seq = 0, at = token;
-    if (a.starts == nullptr) {
-        seq = token / a.tokens;
-        at = token - seq * a.tokens;
-    } else if (token < __ldg(a.starts) || token >= __ldg(a.starts + a.seqs)) {
-        return;  // in no sequence: left as it was
-    }
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_lse[s * a.rows_total + row]);
-    float sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < a.splits; ++s) {
-        const float x = a.part_lse[s * a.rows_total + row];
-        if (x == -INFINITY) continue;
-        const float f = exp2f(x - top);
-        const float4 v = *reinterpret_cast<const float4*>(a.part_o + (s * a.rows_total + row) * 128 + 4 * lane);
-        sum += f;
-        acc.x += f * v.x;
-        acc.y += f * v.y;
-        acc.z += f * v.z;
-        acc.w += f * v.w;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    uint2 pair = make_uint2(Pair<T>::pack(acc.x * inv, acc.y * inv), Pair<T>::pack(acc.z * inv, acc.w * inv));
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + seq * a.o_seq + head * a.o_head + at * a.o_token + 4 * lane) = pair;
-    if (a.lse != nullptr && lane == 0)
-        a.lse[seq * a.l_seq + head * a.l_head + at * a.l_token] = sum == 0.f ? -INFINITY : top + log2f(sum);
-}
-
 template <class T, int MT>
 cudaError_t launch(const ChunkArgs& a, const ChunkMaps& maps, int box_rows, cudaStream_t stream) {
     using L = Layout<MT>;
     auto kernel = chunk_token_kernel<T, MT>;
     cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L::bytes));
     if (err != cudaSuccess) return err;
-    const int64_t rows = static_cast<int64_t>(a.longest) * a.group;
-    int64_t units = a.seqs * ceil_div(rows, L::rows);
-    if (a.starts != nullptr) {  // the tiles of ragged sequences: at most this many
-        const int64_t bound = static_cast<int64_t>(a.tokens) * a.group / L::rows + a.seqs;
-        if (bound < units) units = bound;
-    }
+    const int64_t units = chunk_units(a);
     if (units > 65535 || a.splits > 0x7fffffff) return cudaErrorInvalidConfiguration;
     kernel<<<dim3(a.splits, a.kv_heads, static_cast<unsigned>(units)), kThreads, L::bytes, stream>>>(a, maps, box_rows);
     return cudaGetLastError();
@@ -388,43 +345,10 @@ cudaError_t launch(const ChunkArgs& a, const ChunkMaps& maps, int box_rows, cuda
 
 }  // namespace
 
-void chunk_layout(ChunkArgs& a) {
-    const int rows = static_cast<int64_t>(a.longest) * a.group <= 16 ? 16 : 32;
-    int64_t units = a.seqs * ceil_div(static_cast<int64_t>(a.longest) * a.group, rows);
-    if (a.starts != nullptr) {
-        const int64_t bound = static_cast<int64_t>(a.tokens) * a.group / rows + a.seqs;
-        if (bound < units) units = bound;
-    }
-    // Keys that one row tile can see, in tiles; the lengths themselves are known on the device only.
-    int64_t keys = a.keys;
-    if (a.window != kNoWindow) {
-        const int64_t seen = static_cast<int64_t>(a.window) + a.sinks + a.block + rows + 3 * kKeys;
-        if (seen < keys) keys = seen;
-    }
-    const int64_t tiles = ceil_div(keys, kKeys);
-    // Equal spans: about eight CTAs an SM if every sequence were as long as its table allows, so a
-    // ragged batch still balances; no span under four tiles.
-    const int64_t span = ceil_div(units * a.kv_heads * tiles, 148 * 8);
-    a.span = static_cast<int32_t>(span < 4 ? 4 : span);
-    a.splits = static_cast<int32_t>(ceil_div(tiles, a.span));
-}
-
-int chunk_tile_keys(const ChunkArgs&) { return kKeys; }
-
-cudaError_t launch_chunk(const ChunkArgs& a, const ChunkMaps& maps, bool fp16, int box_rows, cudaStream_t stream) {
-    const bool narrow = static_cast<int64_t>(a.longest) * a.group <= 16;
+cudaError_t launch_chunk_token(const ChunkArgs& a, const ChunkMaps& maps, bool fp16, int box_rows, cudaStream_t stream) {
+    const bool narrow = a.tile_rows == 16;
     if (fp16) return narrow ? launch<half, 1>(a, maps, box_rows, stream) : launch<half, 2>(a, maps, box_rows, stream);
     return narrow ? launch<bf16, 1>(a, maps, box_rows, stream) : launch<bf16, 2>(a, maps, box_rows, stream);
-}
-
-cudaError_t launch_chunk_join(const ChunkArgs& a, bool fp16, cudaStream_t stream) {
-    const int64_t blocks = ceil_div(a.rows_total, 8);
-    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    if (fp16)
-        chunk_join_kernel<half><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
-    else
-        chunk_join_kernel<bf16><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
-    return cudaGetLastError();
 }
 
 }  // namespace abx
