@@ -45,7 +45,8 @@ constexpr int kBarSFree = kBarS + kGroups;       // [group] S(t) is in registers
 constexpr int kBarP = kBarSFree + kGroups;       // [group] P(t) is in shared memory
 constexpr int kBarO = kBarP + kGroups;           // [group] O holds tile t, P(t) is free
 constexpr int kBarDrain = kBarO + kGroups;       // [group]
-constexpr int kNumBars = kBarDrain + kGroups;
+constexpr int kBarTurn = kBarDrain + kGroups;    // [group] the other group is past its exponentials
+constexpr int kNumBars = kBarTurn + kGroups;
 constexpr uint32_t kOffTmem = kOffBars + 8 * kNumBars;
 constexpr uint32_t kOffAbort = kOffTmem + 4;
 constexpr uint32_t kSmemBytes = kOffAbort + 4 + 1024;
@@ -113,6 +114,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             tc::mbar_init(bar(kBarP + g), kGroupRows);
             tc::mbar_init(bar(kBarO + g), 1);
             tc::mbar_init(bar(kBarDrain + g), 1);
+            tc::mbar_init(bar(kBarTurn + g), kGroupRows);
         }
         tc::mbar_init_fence();
     }
@@ -285,13 +287,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     top = max3f(fmaxf(x0, x2), __uint_as_float(r2[31]), __uint_as_float(r3[31]));
                 }
                 const bool grow = (top - m) * a.kappa > kGrow;
-                if (__any_sync(0xffffffffu, grow)) {
+                float shift = mk;
+                if (__any_sync(0xffffffffu, grow || !(fabsf(mk) < kLargeScore))) {
                     const float next = grow ? top : m;
                     const float scale = grow ? exp2f((m - next) * a.kappa) : 1.0f;
                     m = next;
                     mk = m == -INFINITY ? 0.f : m * a.kappa;
                     l *= scale;
-                    if (i > 0) {
+                    if (i > 0 && __any_sync(0xffffffffu, grow)) {
                         if (!tc::mbar_wait_warp_suspend(bar(kBarO + g), (i - 1) & 1, abort_flag, kWaitLimit)) {
                             ok = false;
                             break;
@@ -309,26 +312,36 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                         }
                         tc::tmem_wait_st();
                     }
-                }
-                // x = s * kappa - m * kappa in one FMA. Its rounding is common to the row and falls out of
-                // o = O / l, unless the scores are so large that it reaches whole units.
-                float shift = mk;
-                if (__any_sync(0xffffffffu, !(fabsf(mk) < kLargeScore))) {
-                    const float ref = m == -INFINITY ? 0.f : m;
-                    shift = 0.f;
+                    // x = s * kappa - m * kappa in one FMA. Its rounding is common to the row and falls out of
+                    // o = O / l, unless the scores are so large that it reaches whole units.
+                    shift = mk;
+                    if (!(fabsf(mk) < kLargeScore)) {
+                        shift = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        r0[e] = __float_as_uint(__uint_as_float(r0[e]) - ref);
-                        r1[e] = __float_as_uint(__uint_as_float(r1[e]) - ref);
-                        r2[e] = __float_as_uint(__uint_as_float(r2[e]) - ref);
-                        r3[e] = __float_as_uint(__uint_as_float(r3[e]) - ref);
+                        for (int e = 0; e < 32; ++e) {
+                            r0[e] = __float_as_uint(__uint_as_float(r0[e]) - m);
+                            r1[e] = __float_as_uint(__uint_as_float(r1[e]) - m);
+                            r2[e] = __float_as_uint(__uint_as_float(r2[e]) - m);
+                            r3[e] = __float_as_uint(__uint_as_float(r3[e]) - m);
+                        }
                     }
                 }
-                uint32_t p[64];
+                // P's place is free once the product of the tile before is done.
+                if (i > 0 && !tc::mbar_wait_warp_suspend(bar(kBarO + g), (i - 1) & 1, abort_flag, kWaitLimit)) {
+                    ok = false;
+                    break;
+                }
+                // The groups take turns at the exponential unit: while one's exponentials run, the other
+                // reads, finds maxima and hands over.
+                if (groups == 2 && (g == 1 || i > 0) &&
+                    !tc::mbar_wait_warp_suspend(bar(kBarTurn + g), (g == 1 ? i : i - 1) & 1, abort_flag, kWaitLimit)) {
+                    ok = false;
+                    break;
+                }
                 {
                     const uint64_t kappa2 = pack2(a.kappa, a.kappa), shift2 = pack2(-shift, -shift);
                     uint64_t sum0 = kZeros2, sum1 = kZeros2;
-                    auto weights = [&](const uint32_t (&x)[32], int at) {
+                    auto weights = [&](const uint32_t (&x)[32], uint32_t (&p)[16]) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const uint64_t s2 = (static_cast<uint64_t>(x[2 * e + 1]) << 32) | x[2 * e];
@@ -338,25 +351,28 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                                 sum1 = add2(sum1, pack2(p0, p1));
                             else
                                 sum0 = add2(sum0, pack2(p0, p1));
-                            p[at + e] = Pair<T>::pack(p0, p1);
+                            p[e] = Pair<T>::pack(p0, p1);
                         }
                     };
-                    weights(r0, 0);
-                    weights(r1, 16);
-                    weights(r2, 32);
-                    weights(r3, 48);
+                    auto store = [&](const uint32_t (&p)[16], int quarter) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            *reinterpret_cast<uint4*>(p_row + (quarter >> 1) * kSlab + ((((4 * quarter + c) ^ r) & 7) << 4)) =
+                                make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+                    };
+                    uint32_t p0[16], p1[16];
+                    weights(r0, p0);
+                    store(p0, 0);
+                    weights(r1, p1);
+                    store(p1, 1);
+                    weights(r2, p0);
+                    store(p0, 2);
+                    if (groups == 2) tc::mbar_arrive(bar(kBarTurn + 1 - g));
+                    weights(r3, p1);
+                    store(p1, 3);
                     const float2 y = unpack2(add2(sum0, sum1));
                     l += y.x + y.y;
                 }
-                // P's place is free once the product of the tile before is done.
-                if (i > 0 && !tc::mbar_wait_warp_suspend(bar(kBarO + g), (i - 1) & 1, abort_flag, kWaitLimit)) {
-                    ok = false;
-                    break;
-                }
-#pragma unroll
-                for (int c = 0; c < 16; ++c)
-                    *reinterpret_cast<uint4*>(p_row + (c >> 3) * kSlab + (((c ^ r) & 7) << 4)) =
-                        make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
                 // V rows that no row sees (a page's stale tail) must not meet P = 0 as NaN or infinity. Both
                 // groups clear them, each before its own product.
                 if (!t.any(k0) || !t.any(k0 + kKeys - 1) || (k0 < t.first.low && k0 + kKeys > t.last.sink)) {
