@@ -195,7 +195,6 @@ def dense_cross_attention(q, k, v, *, extra_kv=None, return_lse=False):
     return (out, lse.reshape(batch, heads, tokens)) if return_lse else out
 
 
-@torch.no_grad()
 def window_attention(q, k, v, *, window=None, sinks=0, block=1, return_lse=False):
     """Causal attention (scale 128^-0.5) with a sliding window and sinks over contiguous keys.
 
@@ -208,7 +207,7 @@ def window_attention(q, k, v, *, window=None, sinks=0, block=1, return_lse=False
     long k take the same call. Tiles that no query sees are not read. ``return_lse`` adds the
     base-2 LSE [B,H,N]. `chunk_attention` is the form over a paged cache.
     """
-    if q.device.type == "cpu":
+    if q.is_cpu:
         raise ValueError("B200 attention requires CUDA tensors")
     if window is not None and window < 1:
         raise ValueError("window must be positive, or None")

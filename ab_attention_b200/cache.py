@@ -40,7 +40,6 @@ def kv_cache(pages: int, kv_heads: int, *, page_size: int = 128, dtype=torch.bfl
     return KVCache(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
 
 
-@torch.no_grad()
 def append_kv(cache, k, v, page_table, starts, lengths, *, positions=None, axes=VIDEO_AXES, q=None):
     """Stores the new tokens' k and v [tokens, kv_heads, 128] in their pages, in one launch.
 
@@ -57,7 +56,6 @@ def append_kv(cache, k, v, page_table, starts, lengths, *, positions=None, axes=
     return None if q is None else turned
 
 
-@torch.no_grad()
 def chunk_attention(q, cache, page_table, starts, lengths, *, longest=None, window=None, sinks=0, block=1,
                     return_lse=False, out=None):
     """Attention (scale 128^-0.5) of the new tokens' q [tokens, heads, 128] over the cached keys.

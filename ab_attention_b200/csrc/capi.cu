@@ -753,7 +753,7 @@ int chunk_plan(const abx_chunk_args* c, abx::ChunkArgs& a, size_t& workspace) {
     a.rows_total = all_tokens * c->heads;
     a.kappa = abx::qk_scale_log2();
     abx::chunk_layout(a);
-    workspace = a.splits > 1 ? align_up(static_cast<size_t>(a.splits) * a.rows_total * abx::kHeadDim * 4) +
+    workspace = a.splits > 1 && !a.cluster ? align_up(static_cast<size_t>(a.splits) * a.rows_total * abx::kHeadDim * 4) +
                                    align_up(static_cast<size_t>(a.splits) * a.rows_total * 4)
                              : 0;
     return ABX_OK;
@@ -792,11 +792,12 @@ int abx_rotary(const abx_rotary_args* r, abx_stream_t stream) {
             dims += r->sections[x];
         }
         if (dims != abx::kHeadDim) return fail(ABX_ERR_INVALID_ARGUMENT, "sections must sum to 128 (got %d)", dims);
+        const double log_theta = std::log(r->theta);
         int pair = 0;
         for (int x = 0; x < r->axes; ++x)
             for (int i = 0; i < r->sections[x] / 2; ++i, ++pair) {
                 const double power = r->shared ? 2.0 * pair / abx::kHeadDim : 2.0 * i / r->sections[x];
-                a.freq[pair] = std::pow(r->theta, -power) / 3.14159265358979323846;
+                a.freq[pair] = std::exp(-power * log_theta) / 3.14159265358979323846;
                 a.axis[pair] = static_cast<uint8_t>(x);
             }
     }
@@ -870,7 +871,7 @@ int abx_chunk_attention(const abx_chunk_args* args, void* workspace, size_t work
                             "tensor map of v"))
         return st;
     if (int st = check_cuda(abx::launch_chunk(a, maps, fp16, box_rows, stream), "chunk attention launch")) return st;
-    return a.splits > 1 ? check_cuda(abx::launch_chunk_join(a, fp16, stream), "chunk join launch") : ABX_OK;
+    return need > 0 ? check_cuda(abx::launch_chunk_join(a, fp16, stream), "chunk join launch") : ABX_OK;
 }
 
 }  // extern "C"

@@ -5,43 +5,115 @@ namespace abx {
 namespace {
 
 constexpr int kSms = 148;
+// Below this many parts of one length, at most eight of them form a cluster (no workspace, one launch);
+// from it on, leaving SMs idle would cost more. Four streams of one token over 4,100 keys (9 parts, or 8 in
+// a cluster): 22.5 us joined by a second kernel, 20.6 us in the cluster.
+constexpr int kClusterUpTo = 16;
+// Waves of CTAs for ragged sequences: 48 of up to 16,000 keys take 277 / 266 / 265 / 268 / 282 us with
+// 4 / 6 / 8 / 12 / 20, and 292 us with clusters of 7 equal parts (a cluster waits for its slowest CTA).
+constexpr int kRaggedWaves = 8;
 
-// Joins the splits of each row: o = sum_s 2^(lse_s - lse) o_s. One warp a row, four dims a lane;
-// reads splits * 516 bytes a row.
-template <class T>
+// Joins the splits of each row: o = sum_s 2^(lse_s - lse) o_s. kWarps warps a row, four dims a lane;
+// reads splits * 516 bytes a row. Launched while the splits still run: it waits for them here.
+template <class T, int kWarps>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= a.rows_total) return;
+    __shared__ float4 part[8][32];
+    __shared__ float2 stat[8];
+    cudaGridDependencySynchronize();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int w = warp % kWarps;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (8 / kWarps) + warp / kWarps;
     const int64_t token = row / a.heads;
     const int head = static_cast<int>(row - token * a.heads);
     int64_t seq = 0, at = token;
+    bool mine = row < a.rows_total;
     if (a.starts == nullptr) {
         seq = token / a.tokens;
         at = token - seq * a.tokens;
-    } else if (token < __ldg(a.starts) || token >= __ldg(a.starts + a.seqs)) {
-        return;  // in no sequence: left as it was
+    } else {
+        mine = mine && token >= __ldg(a.starts) && token < __ldg(a.starts + a.seqs);  // else left as it was
     }
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_lse[s * a.rows_total + row]);
-    float sum = 0.f;
+    // This warp's splits w, w + kWarps, ..: 32 at a time, their sums' weights against a running maximum.
+    float top = -INFINITY, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < a.splits; ++s) {
-        const float x = a.part_lse[s * a.rows_total + row];
-        if (x == -INFINITY) continue;
-        const float f = exp2f(x - top);
-        const float4 v = *reinterpret_cast<const float4*>(a.part_o + (s * a.rows_total + row) * 128 + 4 * lane);
-        sum += f;
-        acc.x += f * v.x;
-        acc.y += f * v.y;
-        acc.z += f * v.z;
-        acc.w += f * v.w;
+    if (mine) {
+        for (int base = w; base < a.splits; base += 32 * kWarps) {
+            const int s = base + lane * kWarps;
+            const float x = s < a.splits ? a.part_lse[s * a.rows_total + row] : -INFINITY;
+            float next = x;
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, d));
+            next = fmaxf(next, top);
+            if (next == -INFINITY && !__any_sync(0xffffffffu, isnan(x))) continue;
+            const float scale = next == top ? 1.f : exp2f(top - next), f = exp2f(x - next);  // a NaN stays one
+            top = next;
+            sum = sum * scale + f;
+            acc.x *= scale, acc.y *= scale, acc.z *= scale, acc.w *= scale;
+            const int count = min(32, (a.splits - base + kWarps - 1) / kWarps);
+#pragma unroll 4
+            for (int i = 0; i < count; ++i) {
+                const float4 v = *reinterpret_cast<const float4*>(
+                    a.part_o + (static_cast<int64_t>(base + i * kWarps) * a.rows_total + row) * 128 + 4 * lane);
+                const float fi = __shfl_sync(0xffffffffu, f, i);
+                acc.x += fi * v.x;
+                acc.y += fi * v.y;
+                acc.z += fi * v.z;
+                acc.w += fi * v.w;
+            }
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     }
+    if constexpr (kWarps > 1) {
+        part[warp][lane] = acc;
+        if (lane == 0) stat[warp] = make_float2(top, sum);
+        __syncthreads();
+        if (w != 0) return;
+        float all = -INFINITY;
+        bool reached = false;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            all = fmaxf(all, stat[warp + i].x);
+            reached |= stat[warp + i].y != 0.f;
+        }
+        sum = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (reached) {
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) {
+                const float f = exp2f(stat[warp + i].x - all);
+                const float4 v = part[warp + i][lane];
+                sum += f * stat[warp + i].y;
+                acc.x += f * v.x;
+                acc.y += f * v.y;
+                acc.z += f * v.z;
+                acc.w += f * v.w;
+            }
+        }
+        top = all;
+    }
+    if (!mine) return;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    uint2 pair = make_uint2(Pair<T>::pack(acc.x * inv, acc.y * inv), Pair<T>::pack(acc.z * inv, acc.w * inv));
+    const uint2 pair = make_uint2(Pair<T>::pack(acc.x * inv, acc.y * inv), Pair<T>::pack(acc.z * inv, acc.w * inv));
     *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + seq * a.o_seq + head * a.o_head + at * a.o_token + 4 * lane) = pair;
     if (a.lse != nullptr && lane == 0)
         a.lse[seq * a.l_seq + head * a.l_head + at * a.l_token] = sum == 0.f ? -INFINITY : top + log2f(sum);
+}
+
+template <class T, int kWarps>
+cudaError_t launch_join(const ChunkArgs& a, cudaStream_t stream) {
+    const int64_t blocks = ceil_div(a.rows_total, 8 / kWarps);
+    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(blocks));
+    config.blockDim = dim3(256);
+    config.stream = stream;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, chunk_join_kernel<T, kWarps>, a);
 }
 
 }  // namespace
@@ -66,11 +138,22 @@ void chunk_layout(ChunkArgs& a) {
     }
     const int64_t tiles = ceil_div(keys, tile_keys);
     if (a.tile_rows < 256) {
-        // Equal spans: about eight CTAs an SM if every sequence were as long as its table allows, so a
-        // ragged batch still balances; no span under four tiles.
-        const int64_t span = ceil_div(ctas * tiles, kSms * 8);
-        a.span = static_cast<int32_t>(span < 4 ? 4 : span);
-        a.splits = static_cast<int32_t>(ceil_div(tiles, a.span));
+        // CTAs that fit the GPU at a time, and how many the call should come to: one wave where all sequences
+        // have one length, several where they are ragged (as if all were as long as the table allows: the
+        // lengths are on the device), so that they still balance. No part under four tiles.
+        const int64_t slots = kSms * (a.tile_rows == 16 ? 2 : 1);
+        const bool ragged = a.starts != nullptr && a.seqs > 1;
+        const int64_t most = ceil_div(tiles, 4), want = ragged ? ceil_div(slots * kRaggedWaves, ctas) : slots / ctas;
+        int64_t splits = want < 1 ? 1 : want > most ? most : want;
+        a.span = 0;
+        if (ragged) {  // equal spans, joined through the workspace
+            a.span = static_cast<int32_t>(ceil_div(tiles, splits));
+            splits = ceil_div(tiles, a.span);
+        } else if (splits < kClusterUpTo) {  // equal parts, joined in a cluster
+            splits = splits < kMaxCluster ? splits : kMaxCluster;
+            a.cluster = splits > 1;
+        }
+        a.splits = static_cast<int32_t>(splits);
         return;
     }
     // Equal parts, as many as make the waves of CTAs (one an SM) shortest: a part costs its tiles and
@@ -97,13 +180,10 @@ cudaError_t launch_chunk(const ChunkArgs& a, const ChunkMaps& maps, bool fp16, i
 }
 
 cudaError_t launch_chunk_join(const ChunkArgs& a, bool fp16, cudaStream_t stream) {
-    const int64_t blocks = ceil_div(a.rows_total, 8);
-    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    if (fp16)
-        chunk_join_kernel<half><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
-    else
-        chunk_join_kernel<bf16><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
-    return cudaGetLastError();
+    // A block a row while there are few rows: the splits' loads are what a row waits for.
+    if (a.rows_total <= 8 * kSms)
+        return fp16 ? launch_join<half, 8>(a, stream) : launch_join<bf16, 8>(a, stream);
+    return fp16 ? launch_join<half, 1>(a, stream) : launch_join<bf16, 1>(a, stream);
 }
 
 }  // namespace abx

@@ -40,6 +40,7 @@ struct ChunkArgs {
     int32_t window, sinks, block;  // window: kNoWindow without one
     int32_t tile_rows;     // rows of a tile: 16 or 32 (chunk_token.cu), 256 (chunk_tile.cu)
     int32_t splits;        // CTAs that share the keys of one row tile
+    int32_t cluster;       // 1: the splits of a row tile form a cluster and join their rows themselves
     int32_t span;          // key tiles of one split, or 0: the row tile's keys in equal parts
     int64_t rows_total;    // tokens of all sequences * heads
     float kappa;           // 128^-0.5 * log2(e)
@@ -48,6 +49,7 @@ struct ChunkArgs {
 
 constexpr int32_t kNoWindow = 0x40000000;
 constexpr int32_t kMaxCacheKeys = 0x3fffffff;
+constexpr int kMaxCluster = 8;
 constexpr int kChunkTokenKeys = 64;  // keys of a tile of each kernel
 constexpr int kChunkTileKeys = 128;
 
@@ -195,6 +197,28 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int3
         : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
+// All threads of all CTAs of the cluster; what they wrote before is seen after.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// This CTA's shared address `at`, read in CTA `rank` of the cluster.
+__device__ __forceinline__ float cluster_load(uint32_t at, int rank) {
+    float x;
+    asm volatile("{\n.reg .u32 p;\nmapa.shared::cluster.u32 p, %1, %2;\nld.shared::cluster.f32 %0, [p];\n}\n"
+                 : "=f"(x) : "r"(at), "r"(rank) : "memory");
+    return x;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t at, int rank) {
+    float4 x;
+    asm volatile("{\n.reg .u32 p;\nmapa.shared::cluster.u32 p, %4, %5;\nld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [p];\n}\n"
+                 : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at), "r"(rank) : "memory");
+    return x;
+}
+
 // 16-bit pairs of the two element types.
 template <class T>
 struct Pair;
@@ -204,6 +228,9 @@ struct Pair<bf16> {
         __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
         return *reinterpret_cast<uint32_t*>(&p);
     }
+    static __device__ __forceinline__ float2 unpack(uint32_t x) {
+        return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+    }
 };
 template <>
 struct Pair<half> {
@@ -211,6 +238,7 @@ struct Pair<half> {
         __half2 p = __floats2half2_rn(lo, hi);
         return *reinterpret_cast<uint32_t*>(&p);
     }
+    static __device__ __forceinline__ float2 unpack(uint32_t x) { return __half22float2(*reinterpret_cast<__half2*>(&x)); }
 };
 
 // Chooses the kernel (tile_rows) and the splits of a call.

@@ -101,6 +101,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
     chunk_part(a, t.count, split, begin, end);
     const int n = end - begin;
 
+    cudaTriggerProgrammaticLaunchCompletion();  // the join may come onto the GPU; it waits for this grid's end
     if (tid == 0) {
         *abort_flag = 0;
         for (int st = 0; st < kStages; ++st) {

@@ -5,10 +5,11 @@
 // group. It is bound by reading K and V: a ring of 64-key tiles (32 KB) filled
 // by TMA keeps 64-96 KB in flight per CTA. The four consumer warps
 // take 16 keys of every tile each, with a softmax of their own (running maximum
-// and sum in 32 bits; P rounded to the element type for its product), so the
+// and sum in 32 bits; P goes into its product as two terms of the element type, rounded
+// and rest, which costs nothing next to the reads), so the
 // loop has no barrier among them; they are joined once, at the end, through
-// shared memory. With few sequences the keys are split over CTAs as well and
-// joined by chunk_join_kernel.
+// shared memory. With few sequences the keys are split over CTAs as well, joined
+// in a cluster (up to eight) or by chunk_join_kernel.
 #include <type_traits>
 
 #include "chunk.cuh"
@@ -36,7 +37,7 @@ struct Layout {
     static constexpr uint32_t bars = stats + kWarps * rows * 8;
     static constexpr uint32_t abort_flag = bars + 8 * (3 * kStages);
     static constexpr uint32_t bytes = abort_flag + 16 + 1024;
-    static_assert(kWarps * rows * 128 * 4 <= kStages * kStage, "the join reuses the ring");
+    static_assert((kWarps + 1) * rows * 128 * 4 + rows * 4 <= kStages * kStage, "the join reuses the ring");
 };
 
 template <class T>
@@ -74,13 +75,14 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, kvh = blockIdx.y;
     const ChunkUnit u = chunk_unit(a, blockIdx.z, L::rows);
-    if (u.seq < 0) return;
+    if (u.seq < 0) return;  // past the last tile
     const int rows = min(L::rows, u.n * a.group - u.row0);
     const KeyTiles t = chunk_tiles<kKeys>(a, u, u.row0, u.row0 + rows - 1);
     int begin, end;
     chunk_part(a, t.count, split, begin, end);
     const int n = end - begin;
 
+    cudaTriggerProgrammaticLaunchCompletion();  // the join may come onto the GPU; it waits for this grid's end
     if (tid == 0) {
         *abort_flag = 0;
         for (int st = 0; st < kStages; ++st) {
@@ -90,19 +92,7 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
         }
         tc::mbar_init_fence();
     }
-    // The rows' queries, zeros past the last row.
-    if (n > 0) {
-        for (int i = tid; i < L::rows * 16; i += kThreads) {
-            const int r = i >> 4, c = i & 15;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (r < rows) {
-                const int token = (u.row0 + r) / a.group, head = kvh * a.group + (u.row0 + r) % a.group;
-                x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + u.seq * a.q_seq + head * a.q_head +
-                                                    (u.first + token) * a.q_token + c * 8);
-            }
-            *reinterpret_cast<uint4*>(mem + L::q + chunk_at(r, c, L::rows * 128)) = x;
-        }
-    }
+    if (warp == kWarps && lane < 2) prefetch_map(lane ? &maps.v : &maps.k);
     __syncthreads();
 
     float* stat_m = reinterpret_cast<float*>(mem + L::stats);
@@ -111,9 +101,15 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
     if (warp == kWarps) {
         // ---- loader: one box a lane ----
         const int boxes = kKeys / box_rows;  // of one slab
+        const int op = lane / (2 * boxes), rest = lane % (2 * boxes), slab = rest & 1, box = rest >> 1;
+        const uint32_t to = op * kOperand + slab * kSlab + box * box_rows * 128;
+        auto key = [&](int i) { return t.tile(begin + i) * kKeys + box * box_rows; };
+        int32_t page = lane < 4 * boxes && n > 0 ? chunk_page(a, u, t, key(0), box_rows) : 0;
         int issued = 0;
         for (int i = 0; i < n; ++i) {
             const int st = i % kStages, use = i / kStages;
+            // the next tile's page is looked up while this one waits for its place
+            const int32_t next = lane < 4 * boxes && i + 1 < n ? chunk_page(a, u, t, key(i + 1), box_rows) : 0;
             const bool free_ok =
                 use == 0 || tc::mbar_wait_suspend(empty(st), (use - 1) & 1, abort_flag, kWaitLimit);
             if (!__all_sync(0xffffffffu, free_ok)) break;
@@ -123,15 +119,10 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
                 tc::mbar_arrive_expect_tx(v_full(st), kOperand);
             }
             __syncwarp();
-            const int32_t k0 = t.tile(begin + i) * kKeys;
-            if (lane < 4 * boxes) {
-                const int op = lane / (2 * boxes), rest = lane % (2 * boxes), slab = rest & 1, box = rest >> 1;
-                const int32_t j = k0 + box * box_rows;
-                const int32_t page = chunk_page(a, u, t, j, box_rows);
-                const int32_t y = a.table ? j % a.page_size : j;
-                tma_load_4d(base + st * kStage + op * kOperand + slab * kSlab + box * box_rows * 128,
-                            op ? &maps.v : &maps.k, 64 * slab, y, kvh, page, op ? v_full(st) : k_full(st));
-            }
+            if (lane < 4 * boxes)
+                tma_load_4d(base + st * kStage + to, op ? &maps.v : &maps.k, 64 * slab, a.table ? key(i) % a.page_size : key(i),
+                            kvh, page, op ? v_full(st) : k_full(st));
+            page = next;
             __syncwarp();
         }
         if (lane == 0) {  // every copy has landed before the ring is used for anything else
@@ -159,7 +150,29 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[i][d][e] = 0.f;
         }
+        // The rows' queries, zeros past the last row (the first tiles are on their way meanwhile).
+        if (n > 0) {
+            for (int i = tid; i < L::rows * 16; i += kWarps * 32) {
+                const int r = i >> 4, c = i & 15;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (r < rows) {
+                    const int token = (u.row0 + r) / a.group, head = kvh * a.group + (u.row0 + r) % a.group;
+                    x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + u.seq * a.q_seq + head * a.q_head +
+                                                        (u.first + token) * a.q_token + c * 8);
+                }
+                *reinterpret_cast<uint4*>(mem + L::q + chunk_at(r, c, L::rows * 128)) = x;
+            }
+        }
+        asm volatile("bar.sync 1, %0;\n" ::"n"(kWarps * 32) : "memory");
         const int mat = lane >> 3, mr = lane & 7;
+        auto load_q = [&](uint32_t (&qa)[4], int x, int step) {
+            ldmatrix_x4(qa, base + L::q + chunk_at(16 * x + (mat & 1) * 8 + mr, 2 * step + (mat >> 1), L::rows * 128));
+        };
+        uint32_t q1[MT == 1 ? 8 : 1][4];  // 16 rows stay in registers; 32 are read again for each tile
+        if constexpr (MT == 1) {
+#pragma unroll
+            for (int step = 0; step < 8; ++step) load_q(q1[step], 0, step);
+        }
         for (int i = 0; i < n; ++i) {
             const int st = i % kStages;
             const uint32_t phase = (i / kStages) & 1;
@@ -180,8 +193,9 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
                 ldmatrix_x4(kb, kbase + chunk_at(warp * kWarpKeys + (mat >> 1) * 8 + mr, 2 * step + (mat & 1), kSlab));
 #pragma unroll
                 for (int x = 0; x < MT; ++x) {
-                    uint32_t qa[4];
-                    ldmatrix_x4(qa, base + L::q + chunk_at(16 * x + (mat & 1) * 8 + mr, 2 * step + (mat >> 1), L::rows * 128));
+                    uint32_t q2[4];
+                    if constexpr (MT > 1) load_q(q2, x, step);
+                    const uint32_t (&qa)[4] = MT == 1 ? q1[step] : q2;
                     mma_16816<T>(s[x][0], qa, kb[0], kb[1]);
                     mma_16816<T>(s[x][1], qa, kb[2], kb[3]);
                 }
@@ -199,7 +213,7 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
                             if (!(j < w.end && (j >= w.low || j < w.sink))) s[x][y][e] = -INFINITY;
                         }
             }
-            uint32_t p[MT][4];
+            uint32_t p[MT][4], rest[MT][4];
 #pragma unroll
             for (int x = 0; x < MT; ++x) {
                 // The maximum is kept as the bare score: s - m is exact where it matters, so the
@@ -236,6 +250,8 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
                         const float p1 = exp2f((s[x][y][2 * h + 1] - shift) * a.kappa);
                         l[x][h] += p0 + p1;
                         p[x][2 * y + h] = Pair<T>::pack(p0, p1);
+                        const float2 r = Pair<T>::unpack(p[x][2 * y + h]);
+                        rest[x][2 * y + h] = Pair<T>::pack(p0 - r.x, p1 - r.y);
                     }
                 }
             }
@@ -260,6 +276,8 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
                 for (int x = 0; x < MT; ++x) {
                     mma_16816<T>(o[x][2 * d], p[x], vb[0], vb[1]);
                     mma_16816<T>(o[x][2 * d + 1], p[x], vb[2], vb[3]);
+                    mma_16816<T>(o[x][2 * d], rest[x], vb[0], vb[1]);
+                    mma_16816<T>(o[x][2 * d + 1], rest[x], vb[2], vb[3]);
                 }
             }
             __syncwarp();
@@ -291,6 +309,9 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
                                                2 * (lane & 3)) = make_float2(o[x][d][2 * h], o[x][d][2 * h + 1]);
     }
     __syncthreads();
+    // The CTA's own result, where the other CTAs of its cluster read it.
+    float* share = part + kWarps * L::rows * 128;  // [row][128]
+    float* share_lse = share + L::rows * 128;
     // Join the warps: weight 2^(m_w - m); a row that nothing reached gives zeros and -inf.
     for (int i = tid; i < rows * 32; i += kThreads) {
         const int r = i >> 5, c = (i & 31) * 4;
@@ -315,7 +336,10 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const float lse = sum == 0.f ? -INFINITY : top + log2f(sum);
         const int token = (u.row0 + r) / a.group, head = kvh * a.group + (u.row0 + r) % a.group;
-        if (a.splits > 1) {
+        if (a.cluster) {
+            *reinterpret_cast<float4*>(share + r * 128 + c) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            if (c == 0) share_lse[r] = lse;
+        } else if (a.splits > 1) {
             const int64_t tokens_before = a.starts ? u.first : static_cast<int64_t>(u.seq) * a.tokens;
             const int64_t at = split * a.rows_total + (tokens_before + token) * a.heads + head;
             *reinterpret_cast<float4*>(a.part_o + at * 128 + c) =
@@ -328,6 +352,52 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
             if (a.lse != nullptr && c == 0) a.lse[u.seq * a.l_seq + head * a.l_head + (u.first + token) * a.l_token] = lse;
         }
     }
+    if (a.cluster) {
+        // Up to eight splits form a cluster: its CTAs join the rows over distributed shared memory, each
+        // every splits-th row.
+        cluster_sync();
+        for (int r = split + a.splits * warp; r < rows; r += a.splits * (kWarps + 1)) {
+            const uint32_t at = smem_addr(share + r * 128 + 4 * lane), at_lse = smem_addr(share_lse + r);
+            float lse[kMaxCluster];
+            float4 x[kMaxCluster];
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int s = 0; s < kMaxCluster; ++s)
+                if (s < a.splits) {
+                    lse[s] = cluster_load(at_lse, s);
+                    x[s] = cluster_load4(at, s);
+                }
+            bool reached = false;
+#pragma unroll
+            for (int s = 0; s < kMaxCluster; ++s)
+                if (s < a.splits) {
+                    top = fmaxf(top, lse[s]);
+                    reached |= lse[s] != -INFINITY;  // a NaN reaches too, and stays one
+                }
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (reached) {
+#pragma unroll
+                for (int s = 0; s < kMaxCluster; ++s)
+                    if (s < a.splits) {
+                        const float f = exp2f(lse[s] - top);
+                        sum += f;
+                        acc.x += f * x[s].x;
+                        acc.y += f * x[s].y;
+                        acc.z += f * x[s].z;
+                        acc.w += f * x[s].w;
+                    }
+            }
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const int token = (u.row0 + r) / a.group, head = kvh * a.group + (u.row0 + r) % a.group;
+            *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + u.seq * a.o_seq + head * a.o_head +
+                                      (u.first + token) * a.o_token + 4 * lane) =
+                make_uint2(Pair<T>::pack(acc.x * inv, acc.y * inv), Pair<T>::pack(acc.z * inv, acc.w * inv));
+            if (a.lse != nullptr && lane == 0)
+                a.lse[u.seq * a.l_seq + head * a.l_head + (u.first + token) * a.l_token] =
+                    sum == 0.f ? -INFINITY : top + log2f(sum);
+        }
+        cluster_sync();  // nobody leaves while its rows are read
+    }
     if (tid == 0 && *abort_flag) raise_device_error(a.error, ABX_ERR_DEVICE_TIMEOUT);
 }
 
@@ -339,8 +409,18 @@ cudaError_t launch(const ChunkArgs& a, const ChunkMaps& maps, int box_rows, cuda
     if (err != cudaSuccess) return err;
     const int64_t units = chunk_units(a);
     if (units > 65535 || a.splits > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    kernel<<<dim3(a.splits, a.kv_heads, static_cast<unsigned>(units)), kThreads, L::bytes, stream>>>(a, maps, box_rows);
-    return cudaGetLastError();
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = a.cluster ? a.splits : 1;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(a.splits, a.kv_heads, static_cast<unsigned>(units));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = L::bytes;
+    config.stream = stream;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, a, maps, box_rows);
 }
 
 }  // namespace

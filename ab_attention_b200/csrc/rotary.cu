@@ -8,8 +8,7 @@
 // frequency is taken in 64 bits in units of pi and reduced there (a position of 2^28
 // is off by 2^-23 radians at most), and no table of angles is read from memory.
 // A thread holds the 16-byte chunks l and l + 8 of a row: pairs of neighbours
-// lie inside a chunk, pairs (i, i + 64) in its two chunks. Rows of four heads are
-// in flight at a time. With few tokens the heads are shared out to more thread
+// lie inside a chunk, pairs (i, i + 64) in its two chunks. With few tokens the heads are shared out to more thread
 // groups instead, which then compute the same angles again.
 #include "rotary.cuh"
 
@@ -19,7 +18,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kLanes = 8;                       // threads of a token
 constexpr int kGroups = kThreads / kLanes;
-constexpr int kUnroll = 4;                      // heads in flight
+// Heads in flight, blocks an SM and thread groups an SM, without and with a cache. Measured (us, one
+// B200): 75,600 tokens x 24 heads / 2 x 10,799 x 80 heads / 10,800 x 36 rows into pages: 152 / 146 / 43 for
+// (4, 2, 160), 155 / 156 / 39 for (2, 3, 64); a register limit that spills costs up to 2x.
+constexpr int kUnroll[2] = {4, 2};
+constexpr int kBlocks[2] = {2, 3};
+constexpr int kWant[2] = {160, 64};
 
 template <class T>
 struct Vec {  // eight elements
@@ -83,7 +87,8 @@ __device__ __forceinline__ void turn(Vec<T>& lo, Vec<T>& hi, const float (&cs)[8
 }
 
 template <class T, bool kPaged>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? kBlocks[kPaged] : 1) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+    constexpr int kHeads = kUnroll[kPaged];
     __shared__ double freq[kPairs];
     __shared__ uint8_t axis[kPairs];
     if (threadIdx.x < kPairs) {
@@ -137,35 +142,36 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
         }
     }
 
-    for (int h = h0; h < h1; h += kUnroll) {
-        Vec<T> lo[kUnroll], hi[kUnroll];
-        T* dst[kUnroll];
-        bool turned[kUnroll];
-#pragma unroll
-        for (int i = 0; i < kUnroll; ++i) {
-            dst[i] = nullptr;
-            turned[i] = false;
-            if (h + i >= h1) continue;
-            int head = h + i, j = 0;
-            while (head >= a.job[j].heads) head -= a.job[j++].heads;
-            const RotaryJob& job = a.job[j];
-            if (kPaged && job.paged) {
-                if (page >= 0) dst[i] = static_cast<T*>(job.dst) + page * job.d_batch + head * job.d_head + slot * job.d_token;
-            } else {
-                dst[i] = static_cast<T*>(job.dst) + batch * job.d_batch + head * job.d_head + token * job.d_token;
-            }
-            if (dst[i] == nullptr) continue;
-            turned[i] = job.turn != 0;
-            const T* src = static_cast<const T*>(job.src) + batch * job.s_batch + head * job.s_head + token * job.s_token;
-            lo[i] = load8(src + 8 * lane);
-            hi[i] = load8(src + 64 + 8 * lane);
+    int first = 0;  // head of all jobs that the job starts with
+    for (int j = 0; j < a.jobs; first += a.job[j++].heads) {
+        const RotaryJob& job = a.job[j];
+        const int begin = max(h0 - first, 0), end = min(h1 - first, job.heads);
+        if (begin >= end) continue;
+        const T* src = static_cast<const T*>(job.src) + batch * job.s_batch + begin * job.s_head + token * job.s_token + 8 * lane;
+        T* dst;
+        if (kPaged && job.paged) {
+            if (page < 0) continue;
+            dst = static_cast<T*>(job.dst) + page * job.d_batch + begin * job.d_head + slot * job.d_token + 8 * lane;
+        } else {
+            dst = static_cast<T*>(job.dst) + batch * job.d_batch + begin * job.d_head + token * job.d_token + 8 * lane;
         }
+        for (int h = begin; h < end; h += kHeads) {
+            Vec<T> lo[kHeads], hi[kHeads];
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i) {
-            if (dst[i] == nullptr) continue;
-            if (turned[i]) turn(lo[i], hi[i], cs, sn, a.halves != 0);
-            store8(dst[i] + 8 * lane, lo[i]);
-            store8(dst[i] + 64 + 8 * lane, hi[i]);
+            for (int i = 0; i < kHeads; ++i)
+                if (h + i < end) {
+                    lo[i] = load8(src + i * job.s_head);
+                    hi[i] = load8(src + i * job.s_head + 64);
+                }
+#pragma unroll
+            for (int i = 0; i < kHeads; ++i)
+                if (h + i < end) {
+                    if (job.turn) turn(lo[i], hi[i], cs, sn, a.halves != 0);
+                    store8(dst + i * job.d_head, lo[i]);
+                    store8(dst + i * job.d_head + 64, hi[i]);
+                }
+            src += kHeads * job.s_head;
+            dst += kHeads * job.d_head;
         }
     }
 }
@@ -183,8 +189,8 @@ void launch(const RotaryArgs& a, unsigned blocks, cudaStream_t stream) {
 cudaError_t launch_rotary(const RotaryArgs& args, int dtype, cudaStream_t stream) {
     RotaryArgs a = args;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens;
-    // Enough thread groups for every SM to hold 64 (a quarter of its threads), at most one a head.
-    const int64_t want = ceil_div(148 * 64, rows);
+    // With few tokens the heads are shared out to more thread groups, at most one a head.
+    const int64_t want = ceil_div(148 * kWant[a.table != nullptr], rows);
     a.slices = static_cast<int32_t>(want < 1 ? 1 : want > a.heads ? a.heads : want);
     const int64_t blocks = ceil_div(rows * a.slices, kGroups);
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;

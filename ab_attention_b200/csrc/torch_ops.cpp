@@ -579,3 +579,10 @@ TORCH_LIBRARY_IMPL(ab_attention, Meta, m) {
     m.impl("chunk_attention", &chunk_attention_meta);
     m.impl("window_attention", &window_attention_meta);
 }
+
+// No gradients, as everywhere in the package: the streaming operators pass the autograd keys by, which
+// also spares their callers a no_grad block.
+TORCH_LIBRARY_IMPL(ab_attention, Autograd, m) {
+    for (const char* name : {"rotary", "append", "chunk_attention", "window_attention"})
+        m.impl(name, torch::CppFunction::makeFallthrough());
+}

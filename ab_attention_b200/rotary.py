@@ -42,11 +42,10 @@ def grid_positions(frames: int, height: int, width: int, *, first_frame: int = 0
 
 
 def _on_gpu(x: torch.Tensor) -> None:
-    if x.device.type == "cpu":
+    if x.is_cpu:
         raise ValueError("B200 operators require CUDA tensors")
 
 
-@torch.no_grad()
 def apply_rotary(q, k, positions, axes=VIDEO_AXES, *, inverse=False):
     """Turns q [B, H, N, 128] and k [B, Hk, N, 128] (or None); bf16, fp16 or f32.
 

@@ -213,6 +213,19 @@ def test_large_and_extreme_scores(tokens):
     assert torch.equal(o[0][seen], v[0][:, None, 7].expand(-1, tokens, -1)[seen])
 
 
+@pytest.mark.parametrize("tokens,keys", [(1, 40), (1, 20000), (3, 9000), (40, 700), (300, 3000)])
+def test_nan_in_a_query_stays_in_its_row(tokens, keys):
+    g = gen(keys)
+    q, k, v = normal(g, 1, 4, tokens, 128), normal(g, 1, 2, keys, 128), normal(g, 1, 2, keys, 128)
+    want, want_lse = ab.window_attention(q, k, v, return_lse=True)
+    bad = q.clone()
+    bad[0, 1, tokens // 2, 5] = math.nan
+    o, lse = ab.window_attention(bad, k, v, return_lse=True)
+    assert o[0, 1, tokens // 2].isnan().all() and lse[0, 1, tokens // 2].isnan()
+    o[0, 1, tokens // 2], lse[0, 1, tokens // 2] = want[0, 1, tokens // 2], want_lse[0, 1, tokens // 2]
+    assert torch.equal(o, want) and torch.equal(lse, want_lse)
+
+
 def test_window_attention_of_nothing():
     empty = torch.empty(2, 4, 0, 128, dtype=BF, device="cuda")
     q = torch.randn(2, 4, 3, 128, device="cuda").to(BF)
@@ -416,6 +429,20 @@ def test_append_reports_tokens_without_a_place():
         else:  # the other sequence's tokens are stored
             assert torch.equal(b.keys[b.table[1, 0].item(), :, :3].transpose(0, 1), k[4:])
     assert spoiled == [1, 1, 1, 1]
+
+
+def test_no_gradients():
+    """As everywhere in the package: results do not require grad, whatever the inputs do."""
+    g = gen(12)
+    q = normal(g, 1, 2, 5, 128).requires_grad_()
+    p = torch.zeros(5, 3, dtype=torch.int32, device="cuda")
+    assert not ab.apply_rotary(q, q, p)[0].requires_grad
+    assert not ab.window_attention(q, q, q).requires_grad
+    b = Batch(13, [(3, 20)], 2, 2, 16, BF)
+    k = normal(g, 3, 2, 128).requires_grad_()
+    turned = ab.append_kv(b.cache, k, k, *b.plan, positions=p[:3], q=b.q.requires_grad_())
+    assert not turned.requires_grad and not b.keys.requires_grad
+    assert not ab.chunk_attention(b.q, b.cache, *b.plan).requires_grad
 
 
 # ---- streams, graphs, and a run of them together ---------------------------------------------------------------
