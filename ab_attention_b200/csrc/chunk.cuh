@@ -120,6 +120,22 @@ __device__ __forceinline__ ChunkUnit chunk_unit(const ChunkArgs& a, int u, int t
     return r;
 }
 
+// Token and head of row `row`, then of every `step`-th row after it.
+struct RowWalk {
+    int32_t token, head, group, last, token_step, head_step;
+    __device__ __forceinline__ RowWalk(const ChunkArgs& a, int kvh, int row, int step)
+        : token(row / a.group), head(kvh * a.group + row - token * a.group), group(a.group), last((kvh + 1) * a.group),
+          token_step(step / a.group), head_step(step - token_step * a.group) {}
+    __device__ __forceinline__ void next() {
+        token += token_step;
+        head += head_step;
+        if (head >= last) {
+            head -= group;
+            ++token;
+        }
+    }
+};
+
 // Keys [0, sink) and [low, end) are what a query sees.
 struct Seen {
     int32_t sink, low, end;

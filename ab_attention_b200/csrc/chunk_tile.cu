@@ -215,19 +215,20 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
         const int g_row0 = u.row0 + g * kGroupRows;
         const int g_rows = min(kGroupRows, rows - g * kGroupRows);  // at most 0: the group has no rows
         if (g_rows > 0) {
-            // The rows' queries, 16 threads a row; zeros past the last row.
+            // The rows' queries, 16 threads a row, all loads in flight at once; zeros past the last row.
             if (n > 0) {
-#pragma unroll 4
+                RowWalk at(a, kvh, g_row0 + (r >> 4), 8);
+                const T* q = static_cast<const T*>(a.q) + u.seq * a.q_seq + u.first * a.q_token + (r & 15) * 8;
+                uint4 x[kGroupRows / 8];
+#pragma unroll
                 for (int i = 0; i < kGroupRows / 8; ++i) {
-                    const int row = i * 8 + (r >> 4), c = r & 15;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (row < g_rows) {
-                        const int token = (g_row0 + row) / a.group, head = kvh * a.group + (g_row0 + row) % a.group;
-                        x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + u.seq * a.q_seq + head * a.q_head +
-                                                            (u.first + token) * a.q_token + c * 8);
-                    }
-                    *reinterpret_cast<uint4*>(mem + kOffQ + g * kOperand + (c >> 3) * kSlab + row * 128 + (((c ^ row) & 7) << 4)) = x;
+                    x[i] = make_uint4(0, 0, 0, 0);
+                    if (i * 8 + (r >> 4) < g_rows) x[i] = __ldg(reinterpret_cast<const uint4*>(q + at.head * a.q_head + at.token * a.q_token));
+                    at.next();
                 }
+                uint8_t* to = mem + kOffQ + g * kOperand + ((r & 15) >> 3) * kSlab + (r >> 4) * 128 + (((r ^ (r >> 4)) & 7) << 4);
+#pragma unroll
+                for (int i = 0; i < kGroupRows / 8; ++i) *reinterpret_cast<uint4*>(to + i * 1024) = x[i];
                 tc::fence_proxy_async_smem();
                 tc::mbar_arrive(bar(kBarQ + g));
             }
@@ -397,45 +398,59 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             if (ok && n > 0) ok = tc::mbar_wait_warp_suspend(bar(kBarO + g), (n - 1) & 1, abort_flag, kWaitLimit);
             if (ok) {
                 tc::fence_after_sync();
-                const int row = g_row0 + r;
-                const int64_t token = row / a.group, head = kvh * a.group + row % a.group;
                 const bool none = l == 0.f;
                 const float inv = none ? 0.f : 1.f / l;
                 const float lse = none ? -INFINITY : mk + log2f(l);
                 const int64_t tokens_before = a.starts ? u.first : static_cast<int64_t>(u.seq) * a.tokens;
-                const int64_t at = split * a.rows_total + (tokens_before + token) * a.heads + head;
-                T* out = static_cast<T*>(a.o) + u.seq * a.o_seq + head * a.o_head + (u.first + token) * a.o_token;
-#pragma unroll 1
-                for (int c = 0; c < 128; c += 16) {
-                    uint32_t o[16];
+                const int64_t part = split * a.rows_total + tokens_before * a.heads;
+                if (r < g_rows) {
+                    const RowWalk at(a, kvh, g_row0 + r, 0);
+                    if (a.splits > 1)
+                        a.part_lse[part + static_cast<int64_t>(at.token) * a.heads + at.head] = lse;
+                    else if (a.lse != nullptr)
+                        a.lse[u.seq * a.l_seq + at.head * a.l_head + (u.first + at.token) * a.l_token] = lse;
+                }
+                // A row is a lane here; through shared memory (the group's Q and P are done with) its
+                // columns go out 16 bytes a thread, whole rows at a time.
+                const int shift_rows = a.splits > 1 ? 5 : 4;  // 32 or 16 threads a row
+                const uint32_t q_row = kOffQ + g * kOperand, p_base = kOffP + g * kOperand;
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) {
+                    uint32_t o[32];
                     if (n > 0) {
-                        tc::tmem_ld16(o_col + c, o);
+                        tc::tmem_ld32(o_col + c, o);
                         tc::tmem_wait_ld();
                         tc::tmem_reg_fence(o);
                     }
-                    float y[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) y[e] = none || n == 0 ? 0.f : __uint_as_float(o[e]) * inv;
-                    if (r < g_rows) {
-                        if (a.splits > 1) {
+                    for (int e = 0; e < 32; ++e) o[e] = none || n == 0 ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+                    if (a.splits > 1) {  // f32: columns 0-63 in Q's place, 64-127 in P's, 256 bytes a row
+                        uint8_t* to = mem + (c < 64 ? q_row : p_base) + r * 256;
 #pragma unroll
-                            for (int e = 0; e < 16; e += 4)
-                                *reinterpret_cast<float4*>(a.part_o + at * 128 + c + e) =
-                                    make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
-                        } else {
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<uint4*>(to + (((((c & 32) + e) >> 2) ^ (r & 15)) << 4)) =
+                                make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    } else {
+                        uint8_t* to = mem + p_base + r * 256;
 #pragma unroll
-                            for (int e = 0; e < 16; e += 8)
-                                *reinterpret_cast<uint4*>(out + c + e) =
-                                    make_uint4(Pair<T>::pack(y[e], y[e + 1]), Pair<T>::pack(y[e + 2], y[e + 3]),
-                                               Pair<T>::pack(y[e + 4], y[e + 5]), Pair<T>::pack(y[e + 6], y[e + 7]));
+                        for (int e = 0; e < 32; e += 8) {
+                            auto two = [&](int i) { return Pair<T>::pack(__uint_as_float(o[e + i]), __uint_as_float(o[e + i + 1])); };
+                            *reinterpret_cast<uint4*>(to + ((((c + e) >> 3) ^ (r & 15)) << 4)) = make_uint4(two(0), two(2), two(4), two(6));
                         }
                     }
                 }
-                if (r < g_rows) {
+                asm volatile("bar.sync %0, %1;\n" ::"r"(1 + g), "n"(kGroupRows) : "memory");
+                const int step = kGroupRows >> shift_rows, first = r >> shift_rows, c = r & ((1 << shift_rows) - 1);
+                RowWalk at(a, kvh, g_row0 + first, step);
+#pragma unroll 4
+                for (int row = first; row < g_rows; row += step, at.next()) {
+                    const uint32_t from = (a.splits > 1 && c < 16 ? q_row : p_base) + row * 256 + (((c & 15) ^ (row & 15)) << 4);
+                    const uint4 x = *reinterpret_cast<const uint4*>(mem + from);
                     if (a.splits > 1)
-                        a.part_lse[at] = lse;
-                    else if (a.lse != nullptr)
-                        a.lse[u.seq * a.l_seq + head * a.l_head + (u.first + token) * a.l_token] = lse;
+                        *reinterpret_cast<uint4*>(a.part_o + (part + static_cast<int64_t>(at.token) * a.heads + at.head) * 128 + 4 * c) = x;
+                    else
+                        *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + u.seq * a.o_seq + at.head * a.o_head +
+                                                  (u.first + at.token) * a.o_token + 8 * c) = x;
                 }
             }
         }
