@@ -102,6 +102,21 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
     const int n = end - begin;
 
     cudaTriggerProgrammaticLaunchCompletion();  // the join may come onto the GPU; it waits for this grid's end
+    // The rows' queries, 16 threads a row, all loads in flight at once while the CTA sets up; zeros past
+    // the last row.
+    uint4 q_part[kGroupRows / 8];
+    if (warp < kMmaWarp) {
+        const int row0 = (tid >> 7) * kGroupRows + ((tid & 127) >> 4);
+        RowWalk at(a, kvh, u.row0 + row0, 8);
+        const T* q = static_cast<const T*>(a.q) + u.seq * a.q_seq + u.first * a.q_token + (tid & 15) * 8;
+#pragma unroll
+        for (int i = 0; i < kGroupRows / 8; ++i) {
+            q_part[i] = make_uint4(0, 0, 0, 0);
+            if (n > 0 && row0 + i * 8 < rows)
+                q_part[i] = __ldg(reinterpret_cast<const uint4*>(q + at.head * a.q_head + at.token * a.q_token));
+            at.next();
+        }
+    }
     if (tid == 0) {
         *abort_flag = 0;
         for (int st = 0; st < kStages; ++st) {
@@ -215,20 +230,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
         const int g_row0 = u.row0 + g * kGroupRows;
         const int g_rows = min(kGroupRows, rows - g * kGroupRows);  // at most 0: the group has no rows
         if (g_rows > 0) {
-            // The rows' queries, 16 threads a row, all loads in flight at once; zeros past the last row.
             if (n > 0) {
-                RowWalk at(a, kvh, g_row0 + (r >> 4), 8);
-                const T* q = static_cast<const T*>(a.q) + u.seq * a.q_seq + u.first * a.q_token + (r & 15) * 8;
-                uint4 x[kGroupRows / 8];
-#pragma unroll
-                for (int i = 0; i < kGroupRows / 8; ++i) {
-                    x[i] = make_uint4(0, 0, 0, 0);
-                    if (i * 8 + (r >> 4) < g_rows) x[i] = __ldg(reinterpret_cast<const uint4*>(q + at.head * a.q_head + at.token * a.q_token));
-                    at.next();
-                }
                 uint8_t* to = mem + kOffQ + g * kOperand + ((r & 15) >> 3) * kSlab + (r >> 4) * 128 + (((r ^ (r >> 4)) & 7) << 4);
 #pragma unroll
-                for (int i = 0; i < kGroupRows / 8; ++i) *reinterpret_cast<uint4*>(to + i * 1024) = x[i];
+                for (int i = 0; i < kGroupRows / 8; ++i) *reinterpret_cast<uint4*>(to + i * 1024) = q_part[i];
                 tc::fence_proxy_async_smem();
                 tc::mbar_arrive(bar(kBarQ + g));
             }
@@ -264,6 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 if (k0 + kKeys > lo.end || (k0 < hi.low && k0 + kKeys > lo.sink)) {
                     auto hide = [&](uint32_t (&x)[32], int first) {
                         const uint32_t see = low_bits(mine.end - first) & (~low_bits(mine.low - first) | low_bits(mine.sink - first));
+                        if (__all_sync(0xffffffffu, see == 0xffffffffu)) return;
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
                             if (!(see & (1u << e))) x[e] = 0xff800000u;
@@ -386,8 +392,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     if (!t.any(k0 + r)) {
                         uint8_t* v_row = mem + kOffRing + (item % kStages) * kOperand + r * 128;
 #pragma unroll
-                        for (int c = 0; c < 16; ++c)
-                            *reinterpret_cast<uint4*>(v_row + (c >> 3) * kSlab + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                        for (int c = 0; c < 16; ++c)  // in an order without bank conflicts
+                            *reinterpret_cast<uint4*>(v_row + (c >> 3) * kSlab + (((c ^ r) & 7) << 4)) = make_uint4(0, 0, 0, 0);
                     }
                 }
                 tc::fence_proxy_async_smem();
