@@ -674,25 +674,31 @@ int check_pages(int64_t sequences, int64_t table_width, int64_t page_size, int64
     return ABX_OK;
 }
 
-// [128, tokens, heads, pages] with 64-column x box_rows boxes (128-byte swizzle). A
+// Four dims [128, d1, d2, d3] with strides in elements and 64 x b1 x b2 x 1 boxes, 128-byte swizzle. A
 // dim of one element may have any stride; the map wants one that it can encode.
-cudaError_t encode_cache(CUtensorMap* map, const void* base, bool fp16, int64_t tokens, int64_t heads, int64_t pages,
-                         const int64_t (&stride)[3], uint32_t box_rows) {
+cudaError_t encode_rows4d(CUtensorMap* map, const void* base, bool fp16, const int64_t (&size)[3], const int64_t (&stride)[3],
+                          uint32_t b1, uint32_t b2) {
     auto encode = abx::tensor_map_encoder();
     if (encode == nullptr) return cudaErrorNotSupported;
-    const cuuint64_t dims[4] = {abx::kHeadDim, static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(heads),
-                                static_cast<cuuint64_t>(pages)};
-    const int64_t step[3] = {tokens > 1 ? stride[2] : abx::kHeadDim, heads > 1 ? stride[1] : abx::kHeadDim,
-                             pages > 1 ? stride[0] : abx::kHeadDim};
-    const cuuint64_t bytes[3] = {static_cast<cuuint64_t>(step[0]) * 2, static_cast<cuuint64_t>(step[1]) * 2,
-                                 static_cast<cuuint64_t>(step[2]) * 2};
-    const cuuint32_t box[4] = {64, box_rows, 1, 1};
+    cuuint64_t dims[4] = {abx::kHeadDim}, bytes[3];
+    for (int i = 0; i < 3; ++i) {
+        dims[i + 1] = static_cast<cuuint64_t>(size[i]);
+        bytes[i] = static_cast<cuuint64_t>(size[i] > 1 ? stride[i] : abx::kHeadDim) * 2;
+    }
+    const cuuint32_t box[4] = {64, b1, b2, 1};
     const cuuint32_t ones[4] = {1, 1, 1, 1};
     const CUresult r = encode(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                               const_cast<void*>(base), dims, bytes, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// K or V: [128, tokens of a page, kv_heads, pages] from strides (page, head, token).
+cudaError_t encode_cache(CUtensorMap* map, const void* base, bool fp16, int64_t tokens, int64_t heads, int64_t pages,
+                         const int64_t (&stride)[3], uint32_t box_rows) {
+    const int64_t size[3] = {tokens, heads, pages}, steps[3] = {stride[2], stride[1], stride[0]};
+    return encode_rows4d(map, base, fp16, size, steps, box_rows, 1);
 }
 
 int64_t at_most(int64_t x, int64_t most) { return x < most ? x : most; }
@@ -863,13 +869,20 @@ int abx_chunk_attention(const abx_chunk_args* args, void* workspace, size_t work
     const int tile_keys = abx::chunk_tile_keys(a);
     const int box_rows = a.table == nullptr || a.page_size > tile_keys ? tile_keys : a.page_size;
     const int64_t tokens = a.table == nullptr ? a.keys : a.page_size;
-    abx::ChunkMaps maps;
+    abx::ChunkMaps maps{};
     if (int st = check_cuda(encode_cache(&maps.k, args->k, fp16, tokens, a.kv_heads, a.pages, args->k_stride, box_rows),
                             "tensor map of k"))
         return st;
     if (int st = check_cuda(encode_cache(&maps.v, args->v, fp16, tokens, a.kv_heads, a.pages, args->v_stride, box_rows),
                             "tensor map of v"))
         return st;
+    if (a.tile_rows == 256 && 128 % a.group == 0) {
+        // Queries by TMA where a box holds 128 rows in order; rows that repeat (a stride of 0) or that no map
+        // can describe are loaded one by one.
+        const int64_t size[3] = {a.heads, a.tokens, a.table == nullptr ? a.seqs : 1};
+        const int64_t steps[3] = {a.q_head, a.q_token, a.q_seq};
+        a.q_map = encode_rows4d(&maps.q, args->q, fp16, size, steps, a.group, 128 / a.group) == cudaSuccess;
+    }
     if (int st = check_cuda(abx::launch_chunk(a, maps, fp16, box_rows, stream), "chunk attention launch")) return st;
     return need > 0 ? check_cuda(abx::launch_chunk_join(a, fp16, stream), "chunk join launch") : ABX_OK;
 }

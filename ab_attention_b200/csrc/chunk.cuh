@@ -42,6 +42,7 @@ struct ChunkArgs {
     int32_t splits;        // CTAs that share the keys of one row tile
     int32_t cluster;       // 1: the splits of a row tile form a cluster and join their rows themselves
     int32_t span;          // key tiles of one split, or 0: the row tile's keys in equal parts
+    int32_t q_map;         // 1: maps.q describes the queries (the tile kernel, group divides 128)
     int64_t rows_total;    // tokens of all sequences * heads
     float kappa;           // 128^-0.5 * log2(e)
     int* error;
@@ -202,6 +203,7 @@ __device__ __forceinline__ int32_t chunk_page(const ChunkArgs& a, const ChunkUni
 // Of K and V: [128, tokens of a page, kv_heads, pages], 64 columns x `rows` tokens a box, 128-byte swizzle.
 struct ChunkMaps {
     CUtensorMap k, v;
+    CUtensorMap q;  // [128, heads, tokens, sequences], 64 columns x group heads x 128 / group tokens (with q_map)
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int32_t x, int32_t y, int32_t z, int32_t w,

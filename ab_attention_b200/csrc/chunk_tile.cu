@@ -25,11 +25,13 @@ namespace {
 constexpr int kGroups = 2;
 constexpr int kGroupRows = 128;
 constexpr int kKeys = kChunkTileKeys;
-constexpr int kMmaWarp = 8;   // one warp a group
-constexpr int kLoadWarp = 10;
-constexpr int kThreads = 12 * 32;
-constexpr int kSoftmaxRegs = 208;
-constexpr int kOtherRegs = 72;
+constexpr int kMmaWarp = 8;    // one warp a group
+constexpr int kLoadWarp = 10;  // K and V
+constexpr int kPlanWarp = 11;  // what to do next, and its queries
+constexpr int kOutWarp = 12;   // four warps: finished rows
+constexpr int kThreads = 16 * 32;
+constexpr int kSoftmaxRegs = 200;
+constexpr int kOtherRegs = 56;
 constexpr int kStages = 3;    // 32 KB tiles, K and V in the order of use
 constexpr uint32_t kSlab = 128 * 128;      // 128 rows x 64 columns
 constexpr uint32_t kOperand = 2 * kSlab;
@@ -44,12 +46,30 @@ constexpr int kBarS = kBarQ + kGroups;           // [group] S(t) is in TMEM
 constexpr int kBarSFree = kBarS + kGroups;       // [group] S(t) is in registers
 constexpr int kBarP = kBarSFree + kGroups;       // [group] P(t) is in shared memory
 constexpr int kBarO = kBarP + kGroups;           // [group] O holds tile t, P(t) is free
-constexpr int kBarDrain = kBarO + kGroups;       // [group]
-constexpr int kBarTurn = kBarDrain + kGroups;    // [group] the other group is past its exponentials
-constexpr int kNumBars = kBarTurn + kGroups;
-constexpr uint32_t kOffTmem = kOffBars + 8 * kNumBars;
+constexpr int kBarTurn = kBarO + kGroups;        // [group] the other group is past its exponentials
+constexpr int kBarSum = kBarTurn + kGroups;      // [group] a job's sums are in shared memory
+constexpr int kBarOFree = kBarSum + kGroups;     // [group] ... and its O has been read
+constexpr int kBarQFree = kBarOFree + kGroups;   // [group] a job's last scores are done with the queries
+constexpr int kBarDrain = kBarQFree + kGroups;   // [group]
+constexpr int kBarJob = kBarDrain + kGroups;     // [slot] a job is written
+constexpr int kBarJobFree = kBarJob + 2;         // [slot] ... and done with by all 15 other warps
+constexpr int kBarNext = kBarJobFree + 2;        // the answer to the request for another CTA's place
+constexpr int kNumBars = kBarNext + 1;
+constexpr uint32_t kOffNext = kOffBars + (8 * kNumBars + 15) / 16 * 16;  // 16 bytes: the answer
+constexpr uint32_t kOffJobs = kOffNext + 16;
+
+// One row tile with its part of the keys, as the plan warp writes it for the others.
+struct Job {
+    ChunkUnit u;
+    KeyTiles t;
+    Seen low[kGroups], high[kGroups];  // of the first and last row of each group
+    int32_t kvh, split, rows;
+    int32_t begin, n;                  // key tiles; n < 0: no more jobs
+};
+constexpr uint32_t kOffTmem = kOffJobs + 2 * sizeof(Job);
 constexpr uint32_t kOffAbort = kOffTmem + 4;
-constexpr uint32_t kSmemBytes = kOffAbort + 4 + 1024;
+constexpr uint32_t kOffSums = (kOffAbort + 4 + 15) / 16 * 16;  // [group][row]: m * kappa, l
+constexpr uint32_t kSmemBytes = kOffSums + kGroups * kGroupRows * 8;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory exceeds the per-block limit");
 constexpr uint32_t kTmemColumns = 512;
 __device__ __forceinline__ constexpr uint32_t col_o(int g) { return 128u * static_cast<uint32_t>(g); }
@@ -78,62 +98,72 @@ __device__ __forceinline__ int item_v(int t, int n) { return t + 1 < n ? 2 * t +
 // The lowest x of 32 bits.
 __device__ __forceinline__ uint32_t low_bits(int x) { return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u; }
 
+// Asks for the place of a CTA of this grid that has not started; the 16-byte answer lands at `to`.
+__device__ __forceinline__ void ask_next(uint32_t to, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" ::"r"(to), "r"(bar)
+                 : "memory");
+}
+// The answer: whether there was one, and its block index.
+__device__ __forceinline__ bool read_next(uint32_t from, int& x, int& y, int& z) {
+    uint32_t got, bx, by, bz;
+    asm volatile(
+        "{\n"
+        ".reg .b128 answer;\n"
+        ".reg .pred p;\n"
+        "ld.shared.b128 answer, [%4];\n"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, answer;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "mov.u32 %1, 0;\n"
+        "mov.u32 %2, 0;\n"
+        "mov.u32 %3, 0;\n"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, answer;\n"
+        "}\n"
+        : "=r"(got), "=r"(bx), "=r"(by), "=r"(bz)
+        : "r"(from)
+        : "memory");
+    x = static_cast<int>(bx), y = static_cast<int>(by), z = static_cast<int>(bz);
+    return got != 0;
+}
+
 template <class T>
 __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs a, const __grid_constant__ ChunkMaps maps,
                                                                 const int box_rows) {
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t raw = smem_addr(smem_raw);
-    const uint32_t base = (raw + 1023u) & ~1023u;
-    uint8_t* mem = smem_raw + (base - raw);
+    extern __shared__ __align__(1024) uint8_t mem[];
+    const uint32_t base = smem_addr(mem);
+    if ((base & 1023u) != 0) {  // swizzled tiles start on 1,024 bytes; there is no room to round up
+        if (threadIdx.x == 0) raise_device_error(a.error, ABX_ERR_CUDA);
+        return;
+    }
     auto bar = [&](int i) { return base + kOffBars + 8u * i; };
     volatile int* abort_flag = reinterpret_cast<volatile int*>(mem + kOffAbort);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mem + kOffTmem);
+    Job* jobs = reinterpret_cast<Job*>(mem + kOffJobs);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    // Tiles of rows fastest, then splits, then key heads: CTAs that run at the same time share K and V in L2.
-    const int kvh = blockIdx.z, split = blockIdx.y;
-    const ChunkUnit u = chunk_unit(a, blockIdx.x, kGroups * kGroupRows);
-    if (u.seq < 0) return;
-    const int rows = min(kGroups * kGroupRows, u.n * a.group - u.row0);
-    const int groups = rows > kGroupRows ? 2 : 1;
-    const KeyTiles t = chunk_tiles<kKeys>(a, u, u.row0, u.row0 + rows - 1);
-    int begin, end;
-    chunk_part(a, t.count, split, begin, end);
-    const int n = end - begin;
-
-    cudaTriggerProgrammaticLaunchCompletion();  // the join may come onto the GPU; it waits for this grid's end
-    // The rows' queries, 16 threads a row, all loads in flight at once while the CTA sets up; zeros past
-    // the last row.
-    uint4 q_part[kGroupRows / 8];
-    if (warp < kMmaWarp) {
-        const int row0 = (tid >> 7) * kGroupRows + ((tid & 127) >> 4);
-        RowWalk at(a, kvh, u.row0 + row0, 8);
-        const T* q = static_cast<const T*>(a.q) + u.seq * a.q_seq + u.first * a.q_token + (tid & 15) * 8;
-#pragma unroll
-        for (int i = 0; i < kGroupRows / 8; ++i) {
-            q_part[i] = make_uint4(0, 0, 0, 0);
-            if (n > 0 && row0 + i * 8 < rows)
-                q_part[i] = __ldg(reinterpret_cast<const uint4*>(q + at.head * a.q_head + at.token * a.q_token));
-            at.next();
-        }
-    }
     if (tid == 0) {
         *abort_flag = 0;
         for (int st = 0; st < kStages; ++st) {
             tc::mbar_init(bar(kBarFull + st), 1);
-            tc::mbar_init(bar(kBarEmpty + st), groups);
+            tc::mbar_init(bar(kBarEmpty + st), kGroups);
         }
         for (int g = 0; g < kGroups; ++g) {
-            tc::mbar_init(bar(kBarQ + g), kGroupRows);
+            tc::mbar_init(bar(kBarQ + g), 1);
             tc::mbar_init(bar(kBarS + g), 1);
             tc::mbar_init(bar(kBarSFree + g), kGroupRows);
             tc::mbar_init(bar(kBarP + g), kGroupRows);
             tc::mbar_init(bar(kBarO + g), 1);
-            tc::mbar_init(bar(kBarDrain + g), 1);
             tc::mbar_init(bar(kBarTurn + g), kGroupRows);
+            tc::mbar_init(bar(kBarSum + g), kGroupRows);
+            tc::mbar_init(bar(kBarOFree + g), kGroupRows);
+            tc::mbar_init(bar(kBarQFree + g), 1);
+            tc::mbar_init(bar(kBarDrain + g), 1);
+            tc::mbar_init(bar(kBarJob + g), 1);
+            tc::mbar_init(bar(kBarJobFree + g), 15);
         }
+        tc::mbar_init(bar(kBarNext), 1);
         tc::mbar_init_fence();
     }
+    if (warp == kLoadWarp && lane < (a.q_map ? 3 : 2)) prefetch_map(lane == 0 ? &maps.k : lane == 1 ? &maps.v : &maps.q);
     if (warp == kMmaWarp) {
         tc::tmem_alloc(smem_addr(tmem_slot), kTmemColumns);
         tc::tmem_relinquish();
@@ -142,44 +172,244 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
+    auto wait = [&](int b, int phase) { return tc::mbar_wait_warp_suspend(bar(b), phase & 1, abort_flag, kWaitLimit); };
+    // For waits of a tile's length and more: the warp sleeps through them and leaves the issue slots alone.
+    auto wait_long = [&](int b, int phase) {
+        return tc::mbar_wait_warp(bar(b), phase & 1, abort_flag, kWaitLimit, tc::kLongWaitHintNs);
+    };
+    // The j-th job's slot, once it is written; done_with() gives it back (once a warp).
+    auto job_ready = [&](int j) { return wait_long(kBarJob + (j & 1), j >> 1); };
+    auto done_with = [&](int j) {
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(bar(kBarJobFree + (j & 1)));
+    };
+    // All counters run on over the jobs of the CTA: `ring` K and V tiles, `tiles` key tiles of a group.
 
     if (warp >= kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
-        if (warp == kLoadWarp) {
+        if (warp == kPlanWarp) {
+            // ---- jobs: this CTA's own place in the grid, then the places of CTAs that have not started ----
+            // Tiles of rows fastest, then splits, then key heads: CTAs that run at the same time share K and V in L2.
+            int x = blockIdx.x, y = blockIdx.y, z = blockIdx.z;
+            int asked[kGroups] = {0, 0};  // rounds of queries
+            bool ok = true;
+            for (int j = 0; ok; ++j) {
+                const ChunkUnit u = chunk_unit(a, x, kGroups * kGroupRows);
+                const int rows = u.seq < 0 ? 0 : min(kGroups * kGroupRows, u.n * a.group - u.row0);
+                KeyTiles t{};
+                int begin = 0, end = 0;
+                if (rows > 0) {
+                    t = chunk_tiles<kKeys>(a, u, u.row0, u.row0 + rows - 1);
+                    chunk_part(a, t.count, y, begin, end);
+                }
+                const int n = end - begin, groups = rows > kGroupRows ? 2 : 1;
+                if (j >= 2 && !wait_long(kBarJobFree + (j & 1), (j >> 1) - 1)) break;
+                Job& job = jobs[j & 1];
+                if (lane == 0) {
+                    job.u = u;
+                    job.t = t;
+                    job.kvh = z;
+                    job.split = y;
+                    job.rows = rows;
+                    job.begin = begin;
+                    job.n = n;
+                }
+                if (lane < groups && rows > 0) {
+                    job.low[lane] = chunk_seen(a, u, u.row0 + lane * kGroupRows);
+                    job.high[lane] = chunk_seen(a, u, u.row0 + min((lane + 1) * kGroupRows, rows) - 1);
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    tc::mbar_arrive(bar(kBarJob + (j & 1)));
+                    tc::mbar_arrive_expect_tx(bar(kBarNext), 16);
+                    ask_next(base + kOffNext, bar(kBarNext));
+                }
+                // The rows' queries, as soon as the last scores of the job before are done with theirs: by TMA, or
+                // 16 lanes a row, zeros past the last row (rows past it are never stored).
+                if (n > 0) {
+                    for (int g = 0; g < groups && ok; ++g) {
+                        if (asked[g] > 0 && !wait_long(kBarQFree + g, asked[g] - 1)) {
+                            ok = false;
+                            break;
+                        }
+                        ++asked[g];
+                        if (a.q_map) {  // two boxes: the heads of 128 / group tokens are the rows in order
+                            if (lane == 0) {
+                                tc::mbar_arrive_expect_tx(bar(kBarQ + g), kOperand);
+                                const int32_t token = u.first + (u.row0 + g * kGroupRows) / a.group;
+                                for (int slab = 0; slab < 2; ++slab)
+                                    tma_load_4d(base + kOffQ + g * kOperand + slab * kSlab, &maps.q, 64 * slab, z * a.group, token,
+                                                a.starts ? 0 : u.seq, bar(kBarQ + g));
+                            }
+                            continue;
+                        }
+                        const int c = lane & 15, row0 = g * kGroupRows + (lane >> 4);
+                        RowWalk at(a, z, u.row0 + row0, 2);
+                        const T* q = static_cast<const T*>(a.q) + u.seq * a.q_seq + u.first * a.q_token + c * 8;
+                        const uint32_t to = base + kOffQ + g * kOperand + (c >> 3) * kSlab;
+#pragma unroll 8
+                        for (int i = 0; i < kGroupRows; i += 2, at.next()) {
+                            const int row = i + (lane >> 4);
+                            const bool valid = row0 + i < rows;
+                            tc::cp_async_16_zfill(to + row * 128 + (((c ^ row) & 7) << 4),
+                                                  valid ? q + at.head * a.q_head + at.token * a.q_token : q, valid);
+                        }
+                        cp_async_commit();
+                    }
+                    if (!a.q_map) {
+                        if (ok && groups == 2) {
+                            cp_async_wait<1>();
+                            tc::fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) tc::mbar_arrive(bar(kBarQ));
+                        }
+                        cp_async_wait<0>();
+                        tc::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (ok && lane == 0) tc::mbar_arrive(bar(kBarQ + groups - 1));
+                    }
+                }
+                // the answer is waited for whatever else happened: it is written to shared memory
+                if (!tc::mbar_wait_suspend(bar(kBarNext), j & 1, abort_flag, kWaitLimit, /*honor_abort=*/false)) ok = false;
+                ok = __all_sync(0xffffffffu, ok);
+                const bool more = read_next(base + kOffNext, x, y, z);
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                if (ok && !more) {
+                    if (j >= 1 && !wait_long(kBarJobFree + ((j + 1) & 1), ((j + 1) >> 1) - 1)) break;
+                    if (lane == 0) {
+                        jobs[(j + 1) & 1].n = -1;
+                        tc::mbar_arrive(bar(kBarJob + ((j + 1) & 1)));
+                    }
+                    break;
+                }
+            }
+            // Queries that were asked for have landed before the CTA ends.
+            for (int g = 0; g < kGroups; ++g)
+                if (a.q_map && lane == 0 && asked[g] > 0)
+                    tc::mbar_wait_suspend(bar(kBarQ + g), (asked[g] - 1) & 1, abort_flag, kWaitLimit, /*honor_abort=*/false);
+            __syncwarp();
+        } else if (warp == kLoadWarp) {
             // ---- loader: K and V tiles in the order of use, one box a lane ----
             const int boxes = kKeys / box_rows;  // of a 64-column slab
-            int issued = 0;
-            for (int i = 0; i < 2 * n; ++i) {
-                const int st = i % kStages, use = i / kStages;
-                const bool is_v = i == 2 * n - 1 || (i > 0 && (i & 1) == 0);
-                const int tile = i == 0 ? 0 : i == 2 * n - 1 ? n - 1 : is_v ? i / 2 - 1 : (i + 1) / 2;
-                const int32_t j = t.tile(begin + tile) * kKeys + (lane >> 1) * box_rows;
-                const int32_t page = lane < 2 * boxes ? chunk_page(a, u, t, j, box_rows) : 0;
-                const bool free_ok =
-                    use == 0 || tc::mbar_wait_suspend(bar(kBarEmpty + st), (use - 1) & 1, abort_flag, kWaitLimit);
-                if (!__all_sync(0xffffffffu, free_ok)) break;
-                issued = i + 1;
-                if (lane == 0) tc::mbar_arrive_expect_tx(bar(kBarFull + st), kOperand);
-                __syncwarp();
-                if (lane < 2 * boxes)
-                    tma_load_4d(base + kOffRing + st * kOperand + (lane & 1) * kSlab + (lane >> 1) * box_rows * 128,
-                                is_v ? &maps.v : &maps.k, 64 * (lane & 1), a.table ? j % a.page_size : j, kvh, page,
-                                bar(kBarFull + st));
-                __syncwarp();
+            int ring = 0;
+            bool ok = true;
+            for (int j = 0; ok; ++j) {
+                if (!job_ready(j)) break;
+                const Job& job = jobs[j & 1];
+                const int n = job.n;
+                if (n < 0) break;
+                const ChunkUnit u = job.u;
+                const KeyTiles t = job.t;
+                const int begin = job.begin, kvh = job.kvh;
+                auto key = [&](int i) {
+                    const bool is_v = i == 2 * n - 1 || (i > 0 && (i & 1) == 0);
+                    const int tile = i == 0 ? 0 : i == 2 * n - 1 ? n - 1 : is_v ? i / 2 - 1 : (i + 1) / 2;
+                    return t.tile(begin + tile) * kKeys + (lane >> 1) * box_rows;
+                };
+                auto page_of = [&](int i) { return i < 2 * n && lane < 2 * boxes ? chunk_page(a, u, t, key(i), box_rows) : 0; };
+                int32_t page = page_of(0);
+                for (int i = 0; i < 2 * n; ++i, ++ring) {
+                    const int st = ring % kStages, use = ring / kStages;
+                    const bool is_v = i == 2 * n - 1 || (i > 0 && (i & 1) == 0);
+                    const int32_t next = page_of(i + 1);  // looked up while this tile waits for its place
+                    if (use > 0 && !wait(kBarEmpty + st, use - 1)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) tc::mbar_arrive_expect_tx(bar(kBarFull + st), kOperand);
+                    __syncwarp();
+                    if (lane < 2 * boxes)
+                        tma_load_4d(base + kOffRing + st * kOperand + (lane & 1) * kSlab + (lane >> 1) * box_rows * 128,
+                                    is_v ? &maps.v : &maps.k, 64 * (lane & 1), a.table ? key(i) % a.page_size : key(i), kvh, page,
+                                    bar(kBarFull + st));
+                    page = next;
+                    __syncwarp();
+                }
+                done_with(j);
             }
-            if (lane == 0)
-                for (int st = 0; st < kStages && st < issued; ++st)
-                    tc::mbar_wait_suspend(bar(kBarFull + st), ((issued - 1 - st) / kStages) & 1, abort_flag, kWaitLimit,
+            if (lane == 0)  // every copy has landed before the CTA ends
+                for (int st = 0; st < kStages && st < ring; ++st)
+                    tc::mbar_wait_suspend(bar(kBarFull + st), ((ring - 1 - st) / kStages) & 1, abort_flag, kWaitLimit,
                                           /*honor_abort=*/false);
             __syncwarp();
-        } else if (warp < kMmaWarp + groups && n > 0) {
+        } else if (warp >= kOutWarp) {
+            // ---- finished rows: o = O / l, lse = m * kappa + log2(l); a row that nothing reached gives zeros and
+            // -inf. A row is a lane; the softmax is at the next job meanwhile ----
+            const int r = tid & 127;
+            int tiles[kGroups] = {0, 0}, rounds[kGroups] = {0, 0};
+            bool ok = true;
+            for (int j = 0; ok; ++j) {
+                if (!job_ready(j)) break;
+                const Job& job = jobs[j & 1];
+                const int n = job.n, rows = job.rows;
+                if (n < 0) break;
+                const int32_t first = job.u.first, kvh = job.kvh, row0 = job.u.row0;
+                const int64_t seq = job.u.seq;
+                const int64_t part = job.split * a.rows_total + (a.starts ? first : seq * a.tokens) * a.heads;
+                done_with(j);
+                for (int g = 0; g * kGroupRows < rows; ++g) {
+                    float mk = 0.f, l = 0.f;
+                    if (n > 0) {
+                        if (!wait_long(kBarSum + g, rounds[g]) || !wait_long(kBarO + g, tiles[g] + n - 1)) {
+                            ok = false;
+                            break;
+                        }
+                        tc::fence_after_sync();
+                        const float2 sums = *reinterpret_cast<const float2*>(mem + kOffSums + (g * kGroupRows + r) * 8);
+                        mk = sums.x, l = sums.y;
+                    }
+                    const bool none = l == 0.f, valid = g * kGroupRows + r < rows;
+                    const float inv = none ? 0.f : 1.f / l;
+                    const RowWalk at(a, kvh, row0 + g * kGroupRows + r, 0);
+                    const int64_t part_row = part + static_cast<int64_t>(at.token) * a.heads + at.head;
+                    T* out = static_cast<T*>(a.o) + seq * a.o_seq + at.head * a.o_head + (first + at.token) * a.o_token;
+                    const uint32_t o_col = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + col_o(g);
+#pragma unroll 1
+                    for (int c = 0; c < 128; c += 16) {
+                        uint32_t o[16];
+                        if (n > 0) {
+                            tc::tmem_ld16(o_col + c, o);
+                            tc::tmem_wait_ld();
+                            tc::tmem_reg_fence(o);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = none ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+                        if (valid && a.splits > 1) {
+#pragma unroll
+                            for (int e = 0; e < 16; e += 4)
+                                *reinterpret_cast<uint4*>(a.part_o + part_row * 128 + c + e) =
+                                    make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        } else if (valid) {
+                            auto two = [&](int e) { return Pair<T>::pack(__uint_as_float(o[e]), __uint_as_float(o[e + 1])); };
+                            *reinterpret_cast<uint4*>(out + c) = make_uint4(two(0), two(2), two(4), two(6));
+                            *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(two(8), two(10), two(12), two(14));
+                        }
+                        __syncwarp();  // TMEM is read by whole warps
+                    }
+                    if (n > 0) {
+                        tc::fence_before_sync();
+                        tc::mbar_arrive(bar(kBarOFree + g));
+                        tiles[g] += n;
+                        ++rounds[g];
+                    }
+                    if (valid) {
+                        const float lse = none ? -INFINITY : mk + log2f(l);
+                        if (a.splits > 1)
+                            a.part_lse[part_row] = lse;
+                        else if (a.lse != nullptr)
+                            a.lse[seq * a.l_seq + at.head * a.l_head + (first + at.token) * a.l_token] = lse;
+                    }
+                }
+            }
+            __syncwarp();
+        } else {
             // ---- products of group g: S(t + 1) as soon as S(t) is in registers, then O += P(t) V(t) ----
             const int g = warp - kMmaWarp;
             const uint64_t qdesc = tc::smem_desc(base + kOffQ + g * kOperand, 16, 1024, tc::kSwizzle128B);
             const uint64_t pdesc = tc::smem_desc(base + kOffP + g * kOperand, 16, 1024, tc::kSwizzle128B);
-            auto full = [&](int item) {
-                return tc::mbar_wait_warp_suspend(bar(kBarFull + item % kStages), (item / kStages) & 1, abort_flag, kWaitLimit);
-            };
+            int ring = 0, tiles = 0, rounds = 0;
+            auto full = [&](int item) { return wait(kBarFull + item % kStages, item / kStages); };
             auto issue_s = [&](int item) {
                 const uint64_t kdesc = tc::smem_desc(base + kOffRing + (item % kStages) * kOperand, 16, 1024, tc::kSwizzle128B);
 #pragma unroll
@@ -190,35 +420,51 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 tc::mma_commit_elect(bar(kBarS + g));
                 tc::mma_commit_elect(bar(kBarEmpty + item % kStages));
             };
-            bool ok = tc::mbar_wait_warp_suspend(bar(kBarQ + g), 0, abort_flag, kWaitLimit) && full(0);
-            if (ok) {
-                tc::fence_after_sync();
-                issue_s(0);
-            }
-            for (int i = 0; ok && i < n; ++i) {
-                if (i + 1 < n) {
-                    if (!full(item_k(i + 1)) ||
-                        !tc::mbar_wait_warp_suspend(bar(kBarSFree + g), i & 1, abort_flag, kWaitLimit)) {
+            bool ok = true;
+            for (int j = 0; ok; ++j) {
+                if (!job_ready(j)) break;
+                const int n = jobs[j & 1].n, groups = jobs[j & 1].rows > kGroupRows ? 2 : 1;
+                if (n < 0) break;
+                done_with(j);
+                if (n == 0) continue;
+                if (g >= groups) {  // the tiles of the other group alone
+                    for (int i = 0; i < 2 * n && ok; ++i) {
+                        ok = full(ring + i);
+                        if (ok && lane == 0) tc::mbar_arrive(bar(kBarEmpty + (ring + i) % kStages));
+                    }
+                    ring += 2 * n;
+                    continue;
+                }
+                for (int i = -1; i < n; ++i) {
+                    if (i + 1 < n) {
+                        if ((i < 0 && !wait(kBarQ + g, rounds)) || !full(ring + item_k(i + 1)) ||
+                            (tiles + i >= 0 && !wait(kBarSFree + g, tiles + i))) {
+                            ok = false;
+                            break;
+                        }
+                        tc::fence_after_sync();
+                        issue_s(ring + item_k(i + 1));
+                        if (i + 2 == n) tc::mma_commit_elect(bar(kBarQFree + g));
+                    }
+                    if (i < 0) continue;
+                    const int item = ring + item_v(i, n);
+                    if (!full(item) || (i == 0 && rounds > 0 && !wait(kBarOFree + g, rounds - 1)) || !wait(kBarP + g, tiles + i)) {
                         ok = false;
                         break;
                     }
                     tc::fence_after_sync();
-                    issue_s(item_k(i + 1));
-                }
-                const int item = item_v(i, n);
-                if (!full(item) || !tc::mbar_wait_warp_suspend(bar(kBarP + g), i & 1, abort_flag, kWaitLimit)) {
-                    ok = false;
-                    break;
-                }
-                tc::fence_after_sync();
-                const uint64_t vdesc =
-                    tc::smem_desc(base + kOffRing + (item % kStages) * kOperand, kSlab, 1024, tc::kSwizzle128B);
+                    const uint64_t vdesc =
+                        tc::smem_desc(base + kOffRing + (item % kStages) * kOperand, kSlab, 1024, tc::kSwizzle128B);
 #pragma unroll
-                for (int s = 0; s < 8; ++s)  // 16 keys a step; V rows as they lie (MN-major)
-                    tc::mma_ss_elect(tmem + col_o(g), pdesc + (((s >> 2) * kSlab + (s & 3) * 32) >> 4),
-                                     vdesc + ((s * 16 * 128) >> 4), idesc<T>(1), (i > 0 || s > 0) ? 1u : 0u);
-                tc::mma_commit_elect(bar(kBarO + g));
-                tc::mma_commit_elect(bar(kBarEmpty + item % kStages));
+                    for (int s = 0; s < 8; ++s)  // 16 keys a step; V rows as they lie (MN-major)
+                        tc::mma_ss_elect(tmem + col_o(g), pdesc + (((s >> 2) * kSlab + (s & 3) * 32) >> 4),
+                                         vdesc + ((s * 16 * 128) >> 4), idesc<T>(1), (i > 0 || s > 0) ? 1u : 0u);
+                    tc::mma_commit_elect(bar(kBarO + g));
+                    tc::mma_commit_elect(bar(kBarEmpty + item % kStages));
+                }
+                ring += 2 * n;
+                tiles += n;
+                ++rounds;
             }
             tc::mma_commit_elect(bar(kBarDrain + g));
             if (lane == 0) tc::mbar_wait_suspend(bar(kBarDrain + g), 0, abort_flag, kWaitLimit, /*honor_abort=*/false);
@@ -227,28 +473,34 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
         const int g = warp >> 2, r = tid & 127;
-        const int g_row0 = u.row0 + g * kGroupRows;
-        const int g_rows = min(kGroupRows, rows - g * kGroupRows);  // at most 0: the group has no rows
-        if (g_rows > 0) {
-            if (n > 0) {
-                uint8_t* to = mem + kOffQ + g * kOperand + ((r & 15) >> 3) * kSlab + (r >> 4) * 128 + (((r ^ (r >> 4)) & 7) << 4);
-#pragma unroll
-                for (int i = 0; i < kGroupRows / 8; ++i) *reinterpret_cast<uint4*>(to + i * 1024) = q_part[i];
-                tc::fence_proxy_async_smem();
-                tc::mbar_arrive(bar(kBarQ + g));
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const uint32_t s_col = lane_base + col_s(g), o_col = lane_base + col_o(g);
+        uint8_t* const p_row = mem + kOffP + g * kOperand + r * 128;
+        int ring = 0, tiles = 0, turns = 0, rounds = 0;
+        bool ok = true;
+        for (int j = 0; ok; ++j) {
+            if (!job_ready(j)) break;
+            const Job& job = jobs[j & 1];
+            const int n = job.n;
+            if (n < 0) break;
+            const int groups = job.rows > kGroupRows ? 2 : 1;
+            const int g_row0 = job.u.row0 + g * kGroupRows;
+            const int g_rows = min(kGroupRows, job.rows - g * kGroupRows);
+            if (g_rows <= 0 || n == 0) {  // the group has no rows, or nothing to do for them
+                ring += 2 * n;
+                done_with(j);
+                continue;
             }
-            const Seen mine = chunk_seen(a, u, g_row0 + min(r, g_rows - 1));
-            const Seen lo = chunk_seen(a, u, g_row0), hi = chunk_seen(a, u, g_row0 + g_rows - 1);
-            const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-            const uint32_t s_col = lane_base + col_s(g), o_col = lane_base + col_o(g);
-            uint8_t* p_row = mem + kOffP + g * kOperand + r * 128;
+            const Seen mine = chunk_seen(a, job.u, g_row0 + min(r, g_rows - 1));
+            // Tiles in [whole_low, whole_end) or below whole_sink are seen whole by all rows of the group.
+            const int32_t whole_end = job.low[g].end, whole_low = job.high[g].low, whole_sink = job.low[g].sink;
+            const int32_t head = job.t.head, low = job.t.low - head, begin = job.begin;
             float m = -INFINITY;   // the row's reference, a bare score
             float mk = 0.f;        // m * kappa, 0 while m is -inf
             float l = 0.f;
-            bool ok = true;
             for (int i = 0; i < n; ++i) {
-                const int32_t k0 = t.tile(begin + i) * kKeys;
-                if (!tc::mbar_wait_warp_suspend(bar(kBarS + g), i & 1, abort_flag, kWaitLimit)) {
+                const int32_t k0 = (begin + i < head ? begin + i : low + begin + i) * kKeys;
+                if (!wait(kBarS + g, tiles + i)) {
                     ok = false;
                     break;
                 }
@@ -266,7 +518,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 tc::fence_before_sync();
                 tc::mbar_arrive(bar(kBarSFree + g));
                 // Keys that the row does not see -> -inf (only in tiles that some row does not see whole).
-                if (k0 + kKeys > lo.end || (k0 < hi.low && k0 + kKeys > lo.sink)) {
+                const bool partly = k0 + kKeys > whole_end || (k0 < whole_low && k0 + kKeys > whole_sink);
+                if (partly) {
                     auto hide = [&](uint32_t (&x)[32], int first) {
                         const uint32_t see = low_bits(mine.end - first) & (~low_bits(mine.low - first) | low_bits(mine.sink - first));
                         if (__all_sync(0xffffffffu, see == 0xffffffffu)) return;
@@ -303,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     mk = m == -INFINITY ? 0.f : m * a.kappa;
                     l *= scale;
                     if (i > 0 && __any_sync(0xffffffffu, grow)) {
-                        if (!tc::mbar_wait_warp_suspend(bar(kBarO + g), (i - 1) & 1, abort_flag, kWaitLimit)) {
+                        if (!wait(kBarO + g, tiles + i - 1)) {
                             ok = false;
                             break;
                         }
@@ -335,14 +588,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     }
                 }
                 // P's place is free once the product of the tile before is done.
-                if (i > 0 && !tc::mbar_wait_warp_suspend(bar(kBarO + g), (i - 1) & 1, abort_flag, kWaitLimit)) {
+                if (tiles + i > 0 && !wait(kBarO + g, tiles + i - 1)) {
                     ok = false;
                     break;
                 }
                 // The groups take turns at the exponential unit: while one's exponentials run, the other
                 // reads, finds maxima and hands over.
-                if (groups == 2 && (g == 1 || i > 0) &&
-                    !tc::mbar_wait_warp_suspend(bar(kBarTurn + g), (g == 1 ? i : i - 1) & 1, abort_flag, kWaitLimit)) {
+                if (groups == 2 && turns + i + g > 0 && !wait(kBarTurn + g, turns + i + g - 1)) {
                     ok = false;
                     break;
                 }
@@ -383,9 +635,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 }
                 // V rows that no row sees (a page's stale tail) must not meet P = 0 as NaN or infinity. Both
                 // groups clear them, each before its own product.
-                if (!t.any(k0) || !t.any(k0 + kKeys - 1) || (k0 < t.first.low && k0 + kKeys > t.last.sink)) {
-                    const int item = item_v(i, n);
-                    if (!tc::mbar_wait_warp_suspend(bar(kBarFull + item % kStages), (item / kStages) & 1, abort_flag, kWaitLimit)) {
+                const KeyTiles& t = job.t;
+                if (partly && (!t.any(k0) || !t.any(k0 + kKeys - 1) || (k0 < t.first.low && k0 + kKeys > t.last.sink))) {
+                    const int item = ring + item_v(i, n);
+                    if (!wait(kBarFull + item % kStages, item / kStages)) {
                         ok = false;
                         break;
                     }
@@ -400,65 +653,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 tc::fence_before_sync();
                 tc::mbar_arrive(bar(kBarP + g));
             }
-            // o = O / l, lse = m * kappa + log2(l); a row that nothing reached gives zeros and -inf.
-            if (ok && n > 0) ok = tc::mbar_wait_warp_suspend(bar(kBarO + g), (n - 1) & 1, abort_flag, kWaitLimit);
-            if (ok) {
-                tc::fence_after_sync();
-                const bool none = l == 0.f;
-                const float inv = none ? 0.f : 1.f / l;
-                const float lse = none ? -INFINITY : mk + log2f(l);
-                const int64_t tokens_before = a.starts ? u.first : static_cast<int64_t>(u.seq) * a.tokens;
-                const int64_t part = split * a.rows_total + tokens_before * a.heads;
-                if (r < g_rows) {
-                    const RowWalk at(a, kvh, g_row0 + r, 0);
-                    if (a.splits > 1)
-                        a.part_lse[part + static_cast<int64_t>(at.token) * a.heads + at.head] = lse;
-                    else if (a.lse != nullptr)
-                        a.lse[u.seq * a.l_seq + at.head * a.l_head + (u.first + at.token) * a.l_token] = lse;
-                }
-                // A row is a lane here; through shared memory (the group's Q and P are done with) its
-                // columns go out 16 bytes a thread, whole rows at a time.
-                const int shift_rows = a.splits > 1 ? 5 : 4;  // 32 or 16 threads a row
-                const uint32_t q_row = kOffQ + g * kOperand, p_base = kOffP + g * kOperand;
-#pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    uint32_t o[32];
-                    if (n > 0) {
-                        tc::tmem_ld32(o_col + c, o);
-                        tc::tmem_wait_ld();
-                        tc::tmem_reg_fence(o);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = none || n == 0 ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
-                    if (a.splits > 1) {  // f32: columns 0-63 in Q's place, 64-127 in P's, 256 bytes a row
-                        uint8_t* to = mem + (c < 64 ? q_row : p_base) + r * 256;
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<uint4*>(to + (((((c & 32) + e) >> 2) ^ (r & 15)) << 4)) =
-                                make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                    } else {
-                        uint8_t* to = mem + p_base + r * 256;
-#pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            auto two = [&](int i) { return Pair<T>::pack(__uint_as_float(o[e + i]), __uint_as_float(o[e + i + 1])); };
-                            *reinterpret_cast<uint4*>(to + ((((c + e) >> 3) ^ (r & 15)) << 4)) = make_uint4(two(0), two(2), two(4), two(6));
-                        }
-                    }
-                }
-                asm volatile("bar.sync %0, %1;\n" ::"r"(1 + g), "n"(kGroupRows) : "memory");
-                const int step = kGroupRows >> shift_rows, first = r >> shift_rows, c = r & ((1 << shift_rows) - 1);
-                RowWalk at(a, kvh, g_row0 + first, step);
-#pragma unroll 4
-                for (int row = first; row < g_rows; row += step, at.next()) {
-                    const uint32_t from = (a.splits > 1 && c < 16 ? q_row : p_base) + row * 256 + (((c & 15) ^ (row & 15)) << 4);
-                    const uint4 x = *reinterpret_cast<const uint4*>(mem + from);
-                    if (a.splits > 1)
-                        *reinterpret_cast<uint4*>(a.part_o + (part + static_cast<int64_t>(at.token) * a.heads + at.head) * 128 + 4 * c) = x;
-                    else
-                        *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + u.seq * a.o_seq + at.head * a.o_head +
-                                                  (u.first + at.token) * a.o_token + 8 * c) = x;
-                }
-            }
+            // The job before has had its sums read.
+            if (!ok || (rounds > 0 && !wait(kBarOFree + g, rounds - 1))) break;
+            *reinterpret_cast<float2*>(mem + kOffSums + (g * kGroupRows + r) * 8) = make_float2(mk, l);
+            tc::mbar_arrive(bar(kBarSum + g));
+            ring += 2 * n;
+            tiles += n;
+            if (groups == 2) turns += n;
+            ++rounds;
+            done_with(j);
         }
     }
 

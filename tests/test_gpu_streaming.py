@@ -226,6 +226,34 @@ def test_nan_in_a_query_stays_in_its_row(tokens, keys):
     assert torch.equal(o, want) and torch.equal(lse, want_lse)
 
 
+@pytest.mark.parametrize("heads,kv,tokens,keys,window,sinks,block", [
+    (36, 36, 1500, 1500, 100, 3, 1), (40, 8, 1100, 1400, None, 0, 1), (24, 2, 777, 777, 33, 130, 64), (70, 14, 900, 300, None, 0, 1),
+])
+def test_many_tiles_of_rows(heads, kv, tokens, keys, window, sinks, block):
+    """More row tiles than the GPU holds at a time, so that each CTA works on several, one after the other."""
+    g = gen(heads)
+    q, k, v = normal(g, 2, heads, tokens, 128), normal(g, 2, kv, keys, 128), normal(g, 2, kv, keys, 128)
+    o, lse = ab.window_attention(q, k, v, window=window, sinks=sinks, block=block, return_lse=True)
+    for b in range(2):
+        hold(o[b].transpose(0, 1), lse[b].T, *(x[b].transpose(0, 1) for x in (q, k, v)), window=window, sinks=sinks, block=block)
+    for _ in range(3):
+        again = ab.window_attention(q, k, v, window=window, sinks=sinks, block=block, return_lse=True)
+        assert torch.equal(again[0], o) and torch.equal(again[1], lse)
+
+
+@pytest.mark.parametrize("heads,kv,page", [(16, 16, 16), (20, 4, 64)])
+def test_many_ragged_chunks(heads, kv, page):
+    """The same for ragged chunks: tiles of one group of rows and of two, sequences without keys or tokens among them."""
+    sizes = [((37 * i) % 150, (211 * i) % 700) for i in range(90)] + [(0, 50), (130, 0), (300, 900), (128, 128), (129, 4)]
+    b = Batch(page, sizes, heads, kv, page, BF)
+    rule = {"window": None, "sinks": 0, "block": 1}
+    first = ab.chunk_attention(b.q, b.cache, *b.plan, longest=300, return_lse=True, **rule)
+    b.check(*first, **rule)
+    for _ in range(3):
+        again = ab.chunk_attention(b.q, b.cache, *b.plan, longest=300, return_lse=True, **rule)
+        assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+
+
 def test_window_attention_of_nothing():
     empty = torch.empty(2, 4, 0, 128, dtype=BF, device="cuda")
     q = torch.randn(2, 4, 3, 128, device="cuda").to(BF)
