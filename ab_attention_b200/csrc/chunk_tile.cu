@@ -30,8 +30,9 @@ constexpr int kLoadWarp = 10;  // K and V
 constexpr int kPlanWarp = 11;  // what to do next, and its queries
 constexpr int kOutWarp = 12;   // four warps: finished rows
 constexpr int kThreads = 16 * 32;
-constexpr int kSoftmaxRegs = 200;
-constexpr int kOtherRegs = 56;
+constexpr int kSoftmaxRegs = 176;
+constexpr int kOtherRegs = 80;
+constexpr int kAskAhead = 4;  // tiles before a job's end at which the next is asked for
 constexpr int kStages = 3;    // 32 KB tiles, K and V in the order of use
 constexpr uint32_t kSlab = 128 * 128;      // 128 rows x 64 columns
 constexpr uint32_t kOperand = 2 * kSlab;
@@ -50,7 +51,8 @@ constexpr int kBarTurn = kBarO + kGroups;        // [group] the other group is p
 constexpr int kBarSum = kBarTurn + kGroups;      // [group] a job's sums are in shared memory
 constexpr int kBarOFree = kBarSum + kGroups;     // [group] ... and its O has been read
 constexpr int kBarQFree = kBarOFree + kGroups;   // [group] a job's last scores are done with the queries
-constexpr int kBarDrain = kBarQFree + kGroups;   // [group]
+constexpr int kBarAsk = kBarQFree + kGroups;     // a job is near its end
+constexpr int kBarDrain = kBarAsk + 1;           // [group]
 constexpr int kBarJob = kBarDrain + kGroups;     // [slot] a job is written
 constexpr int kBarJobFree = kBarJob + 2;         // [slot] ... and done with by all 15 other warps
 constexpr int kBarNext = kBarJobFree + 2;        // the answer to the request for another CTA's place
@@ -89,6 +91,10 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+
+__device__ __forceinline__ void store_shared(uint32_t to, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(to), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 // The place of K(t) and V(t) of `n` tiles in the order of use: K0 K1 V0 K2 V1 .. V(n-1).
@@ -161,6 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             tc::mbar_init(bar(kBarJobFree + g), 15);
         }
         tc::mbar_init(bar(kBarNext), 1);
+        tc::mbar_init(bar(kBarAsk), 1);
         tc::mbar_init_fence();
     }
     if (warp == kLoadWarp && lane < (a.q_map ? 3 : 2)) prefetch_map(lane == 0 ? &maps.k : lane == 1 ? &maps.v : &maps.q);
@@ -173,6 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
     tc::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     auto wait = [&](int b, int phase) { return tc::mbar_wait_warp_suspend(bar(b), phase & 1, abort_flag, kWaitLimit); };
+    auto there = [&](int b, int phase) { return __all_sync(0xffffffffu, tc::mbar_try_wait(bar(b), phase & 1)) != 0; };
     // For waits of a tile's length and more: the warp sleeps through them and leaves the issue slots alone.
     auto wait_long = [&](int b, int phase) {
         return tc::mbar_wait_warp(bar(b), phase & 1, abort_flag, kWaitLimit, tc::kLongWaitHintNs);
@@ -219,11 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     job.high[lane] = chunk_seen(a, u, u.row0 + min((lane + 1) * kGroupRows, rows) - 1);
                 }
                 __syncwarp();
-                if (lane == 0) {
-                    tc::mbar_arrive(bar(kBarJob + (j & 1)));
-                    tc::mbar_arrive_expect_tx(bar(kBarNext), 16);
-                    ask_next(base + kOffNext, bar(kBarNext));
-                }
+                if (lane == 0) tc::mbar_arrive(bar(kBarJob + (j & 1)));
                 // The rows' queries, as soon as the last scores of the job before are done with theirs: by TMA, or
                 // 16 lanes a row, zeros past the last row (rows past it are never stored).
                 if (n > 0) {
@@ -269,7 +273,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                         if (ok && lane == 0) tc::mbar_arrive(bar(kBarQ + groups - 1));
                     }
                 }
-                // the answer is waited for whatever else happened: it is written to shared memory
+                // The next job is asked for shortly before this one's end, not sooner: a place taken early would wait
+                // behind this job while other SMs run dry.
+                if (!ok || (n > 0 && !wait_long(kBarAsk, asked[0] - 1))) break;
+                if (lane == 0) {
+                    tc::mbar_arrive_expect_tx(bar(kBarNext), 16);
+                    ask_next(base + kOffNext, bar(kBarNext));
+                }
                 if (!tc::mbar_wait_suspend(bar(kBarNext), j & 1, abort_flag, kWaitLimit, /*honor_abort=*/false)) ok = false;
                 ok = __all_sync(0xffffffffu, ok);
                 const bool more = read_next(base + kOffNext, x, y, z);
@@ -420,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 tc::mma_commit_elect(bar(kBarS + g));
                 tc::mma_commit_elect(bar(kBarEmpty + item % kStages));
             };
-            bool ok = true;
+            bool ok = true, early = false;  // early: S(0) of the job is on its way
             for (int j = 0; ok; ++j) {
                 if (!job_ready(j)) break;
                 const int n = jobs[j & 1].n, groups = jobs[j & 1].rows > kGroupRows ? 2 : 1;
@@ -435,8 +445,29 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     ring += 2 * n;
                     continue;
                 }
-                for (int i = -1; i < n; ++i) {
-                    if (i + 1 < n) {
+                for (int i = early ? 0 : -1; i < n; ++i) {
+                    if (g == 0 && lane == 0 && i == max(n - kAskAhead, 0)) tc::mbar_arrive(bar(kBarAsk));
+                    __syncwarp();
+                    if (i + 1 == n) {
+                        // The first scores of the next job before this one's last product, which still waits for its P:
+                        // if that job, its queries and its first keys are there.
+                        early = false;
+                        if (there(kBarJob + ((j + 1) & 1), (j + 1) >> 1)) {
+                            const int n2 = jobs[(j + 1) & 1].n, groups2 = jobs[(j + 1) & 1].rows > kGroupRows ? 2 : 1;
+                            const int next = ring + 2 * n;
+                            if (n2 > 0 && g < groups2 && there(kBarQ + g, rounds + 1) &&
+                                there(kBarFull + next % kStages, next / kStages)) {
+                                if (!wait(kBarSFree + g, tiles + i)) {
+                                    ok = false;
+                                    break;
+                                }
+                                tc::fence_after_sync();
+                                issue_s(next);
+                                if (n2 == 1) tc::mma_commit_elect(bar(kBarQFree + g));
+                                early = true;
+                            }
+                        }
+                    } else {
                         if ((i < 0 && !wait(kBarQ + g, rounds)) || !full(ring + item_k(i + 1)) ||
                             (tiles + i >= 0 && !wait(kBarSFree + g, tiles + i))) {
                             ok = false;
@@ -475,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
         const int g = warp >> 2, r = tid & 127;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t s_col = lane_base + col_s(g), o_col = lane_base + col_o(g);
-        uint8_t* const p_row = mem + kOffP + g * kOperand + r * 128;
+        const uint32_t p_row = base + kOffP + g * kOperand + r * 128;
         int ring = 0, tiles = 0, turns = 0, rounds = 0;
         bool ok = true;
         for (int j = 0; ok; ++j) {
@@ -617,8 +648,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     auto store = [&](const uint32_t (&p)[16], int quarter) {
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
-                            *reinterpret_cast<uint4*>(p_row + (quarter >> 1) * kSlab + ((((4 * quarter + c) ^ r) & 7) << 4)) =
-                                make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+                            store_shared(p_row + (quarter >> 1) * kSlab + ((((4 * quarter + c) ^ r) & 7) << 4), p[4 * c], p[4 * c + 1],
+                                         p[4 * c + 2], p[4 * c + 3]);
                     };
                     uint32_t p0[16], p1[16];
                     weights(r0, p0);
@@ -643,10 +674,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                         break;
                     }
                     if (!t.any(k0 + r)) {
-                        uint8_t* v_row = mem + kOffRing + (item % kStages) * kOperand + r * 128;
+                        const uint32_t v_row = base + kOffRing + (item % kStages) * kOperand + r * 128;
 #pragma unroll
                         for (int c = 0; c < 16; ++c)  // in an order without bank conflicts
-                            *reinterpret_cast<uint4*>(v_row + (c >> 3) * kSlab + (((c ^ r) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                            store_shared(v_row + (c >> 3) * kSlab + (((c ^ r) & 7) << 4), 0, 0, 0, 0);
                     }
                 }
                 tc::fence_proxy_async_smem();
