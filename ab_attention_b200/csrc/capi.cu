@@ -752,6 +752,9 @@ int chunk_plan(const abx_chunk_args* c, abx::ChunkArgs& a, size_t& workspace) {
     a.keys = static_cast<int32_t>(paged ? c->table_width * c->page_size : c->keys);
     a.table_width = static_cast<int32_t>(paged ? c->table_width : 0);
     a.page_size = static_cast<int32_t>(paged ? c->page_size : 0);
+    a.page_shift = -1;
+    for (int shift = 4; shift < 30; ++shift)
+        if (a.page_size == 1 << shift) a.page_shift = shift;
     a.pages = static_cast<int32_t>(paged ? c->pages : c->sequences);
     a.window = c->window == 0 ? abx::kNoWindow : static_cast<int32_t>(at_most(c->window, largest));
     a.sinks = c->window == 0 ? 0 : static_cast<int32_t>(at_most(c->sinks, largest));

@@ -12,6 +12,7 @@ constexpr int kClusterUpTo = 16;
 // Waves of CTAs for ragged sequences: 48 of up to 16,000 keys take 277 / 266 / 265 / 268 / 282 us with
 // 4 / 6 / 8 / 12 / 20, and 292 us with clusters of 7 equal parts (a cluster waits for its slowest CTA).
 constexpr int kRaggedWaves = 8;
+constexpr int kRaggedJobs = 5;
 
 // Joins the splits of each row: o = sum_s 2^(lse_s - lse) o_s. kWarps warps a row, four dims a lane;
 // reads splits * 516 bytes a row. Launched while the splits still run: it waits for them here.
@@ -33,6 +34,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
     } else {
         mine = mine && token >= __ldg(a.starts) && token < __ldg(a.starts + a.seqs);  // else left as it was
     }
+    if (mine && a.span > 0) mine = a.part_lse[row] != kWhole;  // written by its only split
     // This warp's splits w, w + kWarps, ..: 32 at a time, their sums' weights against a running maximum.
     float top = -INFINITY, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -160,6 +162,14 @@ void chunk_layout(ChunkArgs& a) {
     // about three more to start and end, joining costs a write and a read of each part's rows.
     a.span = 0;
     a.splits = 1;
+    if (a.starts != nullptr && a.seqs > 1) {
+        // Ragged: equal spans, so that the parts of long sequences come to about kRaggedJobs an SM and balance;
+        // a sequence within one span is not joined.
+        const int64_t want = ceil_div(static_cast<int64_t>(kSms) * kRaggedJobs, ctas), most = ceil_div(tiles, 8);
+        a.span = static_cast<int32_t>(ceil_div(tiles, want < most ? want : most));
+        a.splits = static_cast<int32_t>(ceil_div(tiles, a.span));
+        return;
+    }
     double best = 0;
     for (int s = 1; s <= 16 && s <= tiles; ++s) {
         const double waves = static_cast<double>(ceil_div(ctas * s, kSms));

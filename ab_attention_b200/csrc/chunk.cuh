@@ -28,7 +28,7 @@ struct ChunkArgs {
     int64_t o_seq, o_head, o_token;
     int64_t l_seq, l_head, l_token;
     float* part_o;         // [splits, rows_total, 128] f32, normalised by the split's own sum
-    float* part_lse;       // [splits, rows_total] base 2; -inf: the split saw nothing
+    float* part_lse;       // [splits, rows_total] base 2; -inf: the split saw nothing, +inf: see chunk_part
     const int32_t* starts;   // [seqs + 1] or nullptr (every sequence has `tokens` tokens)
     const int32_t* lengths;  // [seqs] or nullptr (every sequence has `keys` keys)
     const int32_t* table;    // [seqs, table_width] or nullptr (sequence s is page s)
@@ -37,6 +37,7 @@ struct ChunkArgs {
     int32_t longest;       // tokens of the longest sequence
     int32_t keys;          // per sequence, or, paged, at most (table_width * page_size)
     int32_t table_width, page_size, pages;
+    int32_t page_shift;    // log2 of page_size, -1: not a power of two
     int32_t window, sinks, block;  // window: kNoWindow without one
     int32_t tile_rows;     // rows of a tile: 16 or 32 (chunk_token.cu), 256 (chunk_tile.cu)
     int32_t splits;        // CTAs that share the keys of one row tile
@@ -175,14 +176,18 @@ __device__ __forceinline__ KeyTiles chunk_tiles(const ChunkArgs& a, const ChunkU
     return t;
 }
 
-// The part [begin, end) of `count` key tiles that split `s` takes.
-__device__ __forceinline__ void chunk_part(const ChunkArgs& a, int count, int s, int& begin, int& end) {
+// The part [begin, end) of `count` key tiles that split `s` takes. Returns whether the first split
+// has them all: it then writes the result itself and kWhole as its partial lse, and the others write nothing.
+constexpr float kWhole = INFINITY;
+__device__ __forceinline__ bool chunk_part(const ChunkArgs& a, int count, int s, int& begin, int& end) {
     if (a.span > 0) {
         begin = min(s * a.span, count);
         end = min(begin + a.span, count);
+        return count <= a.span;
     } else {
         begin = static_cast<int>(static_cast<int64_t>(count) * s / a.splits);
         end = static_cast<int>(static_cast<int64_t>(count) * (s + 1) / a.splits);
+        return a.splits == 1;
     }
 }
 
@@ -192,12 +197,18 @@ __device__ __forceinline__ int32_t chunk_page(const ChunkArgs& a, const ChunkUni
                                               int32_t box) {
     if (a.table == nullptr) return u.seq;
     if (j >= t.last.end || (j + box <= t.first.low && j >= t.last.sink)) return a.pages;
-    const int32_t page = __ldg(a.table + static_cast<int64_t>(u.seq) * a.table_width + j / a.page_size);
+    const int32_t at = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
+    const int32_t page = __ldg(a.table + static_cast<int64_t>(u.seq) * a.table_width + at);
     if (page < 0 || page >= a.pages) {
         raise_device_error(a.error, ABX_ERR_INVALID_ARGUMENT);
         return a.pages;
     }
     return page;
+}
+
+// The row of key j in its page.
+__device__ __forceinline__ int32_t chunk_page_row(const ChunkArgs& a, int32_t j) {
+    return a.table == nullptr ? j : a.page_shift >= 0 ? j & (a.page_size - 1) : j % a.page_size;
 }
 
 // Of K and V: [128, tokens of a page, kv_heads, pages], 64 columns x `rows` tokens a box, 128-byte swizzle.

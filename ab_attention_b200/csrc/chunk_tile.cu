@@ -65,7 +65,7 @@ struct Job {
     ChunkUnit u;
     KeyTiles t;
     Seen low[kGroups], high[kGroups];  // of the first and last row of each group
-    int32_t kvh, split, rows;
+    int32_t kvh, split, rows, whole;
     int32_t begin, n;                  // key tiles; n < 0: no more jobs
 };
 constexpr uint32_t kOffTmem = kOffJobs + 2 * sizeof(Job);
@@ -203,12 +203,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             bool ok = true;
             for (int j = 0; ok; ++j) {
                 const ChunkUnit u = chunk_unit(a, x, kGroups * kGroupRows);
-                const int rows = u.seq < 0 ? 0 : min(kGroups * kGroupRows, u.n * a.group - u.row0);
+                int rows = u.seq < 0 ? 0 : min(kGroups * kGroupRows, u.n * a.group - u.row0);
                 KeyTiles t{};
                 int begin = 0, end = 0;
+                bool whole = false;
                 if (rows > 0) {
                     t = chunk_tiles<kKeys>(a, u, u.row0, u.row0 + rows - 1);
-                    chunk_part(a, t.count, y, begin, end);
+                    whole = chunk_part(a, t.count, y, begin, end);
+                    if (whole && y > 0) rows = 0;  // nothing to do
                 }
                 const int n = end - begin, groups = rows > kGroupRows ? 2 : 1;
                 if (j >= 2 && !wait_long(kBarJobFree + (j & 1), (j >> 1) - 1)) break;
@@ -219,6 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     job.kvh = z;
                     job.split = y;
                     job.rows = rows;
+                    job.whole = whole;
                     job.begin = begin;
                     job.n = n;
                 }
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     __syncwarp();
                     if (lane < 2 * boxes)
                         tma_load_4d(base + kOffRing + st * kOperand + (lane & 1) * kSlab + (lane >> 1) * box_rows * 128,
-                                    is_v ? &maps.v : &maps.k, 64 * (lane & 1), a.table ? key(i) % a.page_size : key(i), kvh, page,
+                                    is_v ? &maps.v : &maps.k, 64 * (lane & 1), chunk_page_row(a, key(i)), kvh, page,
                                     bar(kBarFull + st));
                     page = next;
                     __syncwarp();
@@ -353,6 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 if (!job_ready(j)) break;
                 const Job& job = jobs[j & 1];
                 const int n = job.n, rows = job.rows;
+                const bool whole = job.whole != 0;
                 if (n < 0) break;
                 const int32_t first = job.u.first, kvh = job.kvh, row0 = job.u.row0;
                 const int64_t seq = job.u.seq;
@@ -385,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                         }
 #pragma unroll
                         for (int e = 0; e < 16; ++e) o[e] = none ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
-                        if (valid && a.splits > 1) {
+                        if (valid && !whole) {
 #pragma unroll
                             for (int e = 0; e < 16; e += 4)
                                 *reinterpret_cast<uint4*>(a.part_o + part_row * 128 + c + e) =
@@ -405,9 +409,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     }
                     if (valid) {
                         const float lse = none ? -INFINITY : mk + log2f(l);
-                        if (a.splits > 1)
-                            a.part_lse[part_row] = lse;
-                        else if (a.lse != nullptr)
+                        if (a.splits > 1) a.part_lse[part_row] = whole ? kWhole : lse;
+                        if (whole && a.lse != nullptr)
                             a.lse[seq * a.l_seq + at.head * a.l_head + (first + at.token) * a.l_token] = lse;
                     }
                 }

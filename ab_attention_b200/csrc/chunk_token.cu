@@ -79,7 +79,8 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
     const int rows = min(L::rows, u.n * a.group - u.row0);
     const KeyTiles t = chunk_tiles<kKeys>(a, u, u.row0, u.row0 + rows - 1);
     int begin, end;
-    chunk_part(a, t.count, split, begin, end);
+    const bool whole = chunk_part(a, t.count, split, begin, end);
+    if (whole && split > 0) return;
     const int n = end - begin;
 
     cudaTriggerProgrammaticLaunchCompletion();  // the join may come onto the GPU; it waits for this grid's end
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
             }
             __syncwarp();
             if (lane < 4 * boxes)
-                tma_load_4d(base + st * kStage + to, op ? &maps.v : &maps.k, 64 * slab, a.table ? key(i) % a.page_size : key(i),
+                tma_load_4d(base + st * kStage + to, op ? &maps.v : &maps.k, 64 * slab, chunk_page_row(a, key(i)),
                             kvh, page, op ? v_full(st) : k_full(st));
             page = next;
             __syncwarp();
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
         if (a.cluster) {
             *reinterpret_cast<float4*>(share + r * 128 + c) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
             if (c == 0) share_lse[r] = lse;
-        } else if (a.splits > 1) {
+        } else if (!whole) {
             const int64_t tokens_before = a.starts ? u.first : static_cast<int64_t>(u.seq) * a.tokens;
             const int64_t at = split * a.rows_total + (tokens_before + token) * a.heads + head;
             *reinterpret_cast<float4*>(a.part_o + at * 128 + c) =
@@ -350,6 +351,7 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
             *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + u.seq * a.o_seq + head * a.o_head +
                                       (u.first + token) * a.o_token + c) = pair;
             if (a.lse != nullptr && c == 0) a.lse[u.seq * a.l_seq + head * a.l_head + (u.first + token) * a.l_token] = lse;
+            if (a.splits > 1 && c == 0) a.part_lse[static_cast<int64_t>(u.first + token) * a.heads + head] = kWhole;
         }
     }
     if (a.cluster) {
