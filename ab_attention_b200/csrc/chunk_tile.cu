@@ -26,23 +26,25 @@ constexpr int kGroups = 2;
 constexpr int kGroupRows = 128;
 constexpr int kKeys = kChunkTileKeys;
 constexpr int kMmaWarp = 8;    // one warp a group
-constexpr int kLoadWarp = 10;  // K and V
-constexpr int kPlanWarp = 11;  // what to do next, and its queries
-constexpr int kOutWarp = 12;   // four warps: finished rows
+constexpr int kLoadWarp = 10;  // one for K, one for V
+constexpr int kOutWarp = 12;   // four warps: finished rows; the first also finds the next job and loads its queries
 constexpr int kThreads = 16 * 32;
 constexpr int kSoftmaxRegs = 176;
 constexpr int kOtherRegs = 80;
 constexpr int kAskAhead = 4;  // tiles before a job's end at which the next is asked for
-constexpr int kStages = 3;    // 32 KB tiles, K and V in the order of use
+constexpr int kVStages = 2;    // K has one: both groups are soon done with it
 constexpr uint32_t kSlab = 128 * 128;      // 128 rows x 64 columns
 constexpr uint32_t kOperand = 2 * kSlab;
 constexpr uint32_t kOffQ = 0;
 constexpr uint32_t kOffP = kOffQ + kGroups * kOperand;
-constexpr uint32_t kOffRing = kOffP + kGroups * kOperand;
-constexpr uint32_t kOffBars = kOffRing + kStages * kOperand;
-constexpr int kBarFull = 0;
-constexpr int kBarEmpty = kBarFull + kStages;
-constexpr int kBarQ = kBarEmpty + kStages;       // [group] the rows' queries are in shared memory
+constexpr uint32_t kOffK = kOffP + kGroups * kOperand;
+constexpr uint32_t kOffV = kOffK + kOperand;
+constexpr uint32_t kOffBars = kOffV + kVStages * kOperand;
+constexpr int kBarK = 0;                         // K(t) is in shared memory
+constexpr int kBarKFree = 1;                     // ... and read by both groups
+constexpr int kBarV = 2;                         // [stage] the same of V(t)
+constexpr int kBarVFree = kBarV + kVStages;      // [stage]
+constexpr int kBarQ = kBarVFree + kVStages;      // [group] the rows' queries are in shared memory
 constexpr int kBarS = kBarQ + kGroups;           // [group] S(t) is in TMEM
 constexpr int kBarSFree = kBarS + kGroups;       // [group] S(t) is in registers
 constexpr int kBarP = kBarSFree + kGroups;       // [group] P(t) is in shared memory
@@ -54,13 +56,13 @@ constexpr int kBarQFree = kBarOFree + kGroups;   // [group] a job's last scores 
 constexpr int kBarAsk = kBarQFree + kGroups;     // a job is near its end
 constexpr int kBarDrain = kBarAsk + 1;           // [group]
 constexpr int kBarJob = kBarDrain + kGroups;     // [slot] a job is written
-constexpr int kBarJobFree = kBarJob + 2;         // [slot] ... and done with by all 15 other warps
+constexpr int kBarJobFree = kBarJob + 2;         // [slot] ... and done with by all 16 warps
 constexpr int kBarNext = kBarJobFree + 2;        // the answer to the request for another CTA's place
 constexpr int kNumBars = kBarNext + 1;
 constexpr uint32_t kOffNext = kOffBars + (8 * kNumBars + 15) / 16 * 16;  // 16 bytes: the answer
 constexpr uint32_t kOffJobs = kOffNext + 16;
 
-// One row tile with its part of the keys, as the plan warp writes it for the others.
+// One row tile with its part of the keys, as the first output warp writes it for all.
 struct Job {
     ChunkUnit u;
     KeyTiles t;
@@ -96,10 +98,6 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
 __device__ __forceinline__ void store_shared(uint32_t to, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(to), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-
-// The place of K(t) and V(t) of `n` tiles in the order of use: K0 K1 V0 K2 V1 .. V(n-1).
-__device__ __forceinline__ int item_k(int t) { return t == 0 ? 0 : 2 * t - 1; }
-__device__ __forceinline__ int item_v(int t, int n) { return t + 1 < n ? 2 * t + 2 : 2 * n - 1; }
 
 // The lowest x of 32 bits.
 __device__ __forceinline__ uint32_t low_bits(int x) { return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u; }
@@ -148,9 +146,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
 
     if (tid == 0) {
         *abort_flag = 0;
-        for (int st = 0; st < kStages; ++st) {
-            tc::mbar_init(bar(kBarFull + st), 1);
-            tc::mbar_init(bar(kBarEmpty + st), kGroups);
+        tc::mbar_init(bar(kBarK), 1);
+        tc::mbar_init(bar(kBarKFree), kGroups);
+        for (int st = 0; st < kVStages; ++st) {
+            tc::mbar_init(bar(kBarV + st), 1);
+            tc::mbar_init(bar(kBarVFree + st), kGroups);
         }
         for (int g = 0; g < kGroups; ++g) {
             tc::mbar_init(bar(kBarQ + g), 1);
@@ -164,13 +164,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             tc::mbar_init(bar(kBarQFree + g), 1);
             tc::mbar_init(bar(kBarDrain + g), 1);
             tc::mbar_init(bar(kBarJob + g), 1);
-            tc::mbar_init(bar(kBarJobFree + g), 15);
+            tc::mbar_init(bar(kBarJobFree + g), 16);
         }
         tc::mbar_init(bar(kBarNext), 1);
         tc::mbar_init(bar(kBarAsk), 1);
         tc::mbar_init_fence();
     }
-    if (warp == kLoadWarp && lane < (a.q_map ? 3 : 2)) prefetch_map(lane == 0 ? &maps.k : lane == 1 ? &maps.v : &maps.q);
+    if (warp == kOutWarp && lane < (a.q_map ? 3 : 2)) prefetch_map(lane == 0 ? &maps.k : lane == 1 ? &maps.v : &maps.q);
     if (warp == kMmaWarp) {
         tc::tmem_alloc(smem_addr(tmem_slot), kTmemColumns);
         tc::tmem_relinquish();
@@ -191,17 +191,68 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(kBarJobFree + (j & 1)));
     };
-    // All counters run on over the jobs of the CTA: `ring` K and V tiles, `tiles` key tiles of a group.
+    // All counters run on over the jobs of the CTA: `keys` key tiles, `tiles` those of a group, `rounds` its jobs.
 
     if (warp >= kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
-        if (warp == kPlanWarp) {
-            // ---- jobs: this CTA's own place in the grid, then the places of CTAs that have not started ----
-            // Tiles of rows fastest, then splits, then key heads: CTAs that run at the same time share K and V in L2.
-            int x = blockIdx.x, y = blockIdx.y, z = blockIdx.z;
-            int asked[kGroups] = {0, 0};  // rounds of queries
+        if (warp >= kLoadWarp && warp < kOutWarp) {
+            // ---- loaders of K and of V; lane b looks up the page of box b ----
+            const bool is_v = warp > kLoadWarp;
+            const CUtensorMap* const map = is_v ? &maps.v : &maps.k;
+            const int boxes = kKeys / box_rows;  // of a 64-column slab
+            int keys = 0;
             bool ok = true;
             for (int j = 0; ok; ++j) {
+                if (!job_ready(j)) break;
+                const Job& job = jobs[j & 1];
+                const int n = job.n;
+                if (n < 0) break;
+                const ChunkUnit u = job.u;
+                const KeyTiles t = job.t;
+                const int begin = job.begin, kvh = job.kvh;
+                done_with(j);
+                int32_t page = 0, row = 0;
+                auto look_up = [&](int i) {
+                    const int32_t k0 = t.tile(begin + i) * kKeys;
+                    page = lane < boxes ? chunk_page(a, u, t, k0 + lane * box_rows, box_rows) : 0;
+                    // a page of 128 keys and less is a box of its own and starts at its first row
+                    row = boxes > 1 ? 0 : chunk_page_row(a, k0);
+                };
+                if (n > 0) look_up(0);
+                for (int i = 0; i < n; ++i, ++keys) {
+                    const int st = is_v ? keys % kVStages : 0, use = is_v ? keys / kVStages : keys;
+                    if (use > 0 && !wait((is_v ? kBarVFree : kBarKFree) + st, use - 1)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t to = base + (is_v ? kOffV : kOffK) + st * kOperand, full = bar((is_v ? kBarV : kBarK) + st);
+                    if (lane == 0) tc::mbar_arrive_expect_tx(full, kOperand);
+                    __syncwarp();
+                    for (int b = 0; b < boxes; ++b) {
+                        const int32_t p = __shfl_sync(0xffffffffu, page, b);
+                        tma_load_4d_elect(to + b * box_rows * 128, map, 0, row, kvh, p, full);
+                        tma_load_4d_elect(to + kSlab + b * box_rows * 128, map, 64, row, kvh, p, full);
+                    }
+                    if (i + 1 < n) look_up(i + 1);  // while that tile's place is still taken
+                }
+            }
+            // Every copy has landed before the CTA ends.
+            if (lane == 0) {
+                if (!is_v && keys > 0)
+                    tc::mbar_wait_suspend(bar(kBarK), (keys - 1) & 1, abort_flag, kWaitLimit, /*honor_abort=*/false);
+                for (int x = max(keys - kVStages, 0); is_v && x < keys; ++x)
+                    tc::mbar_wait_suspend(bar(kBarV + x % kVStages), (x / kVStages) & 1, abort_flag, kWaitLimit,
+                                          /*honor_abort=*/false);
+            }
+            __syncwarp();
+        } else if (warp >= kOutWarp) {
+            // ---- the first of them: jobs. This CTA's own place in the grid, then the places of CTAs that have not
+            // started. Tiles of rows fastest, then splits, then key heads: CTAs that run at the same time share K and
+            // V in L2 ----
+            int x = blockIdx.x, y = blockIdx.y, z = blockIdx.z;
+            int asked[kGroups] = {0, 0};  // rounds of queries
+            int now = 0;                  // key tiles of the latest job
+            auto publish = [&](int j) {
                 const ChunkUnit u = chunk_unit(a, x, kGroups * kGroupRows);
                 int rows = u.seq < 0 ? 0 : min(kGroups * kGroupRows, u.n * a.group - u.row0);
                 KeyTiles t{};
@@ -212,8 +263,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     whole = chunk_part(a, t.count, y, begin, end);
                     if (whole && y > 0) rows = 0;  // nothing to do
                 }
-                const int n = end - begin, groups = rows > kGroupRows ? 2 : 1;
-                if (j >= 2 && !wait_long(kBarJobFree + (j & 1), (j >> 1) - 1)) break;
+                const int n = rows > 0 ? end - begin : 0, groups = rows > kGroupRows ? 2 : 1;
+                now = n;
+                if (j >= 2 && !wait_long(kBarJobFree + (j & 1), (j >> 1) - 1)) return false;
                 Job& job = jobs[j & 1];
                 if (lane == 0) {
                     job.u = u;
@@ -231,127 +283,75 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 }
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(bar(kBarJob + (j & 1)));
+                if (n == 0) return true;
                 // The rows' queries, as soon as the last scores of the job before are done with theirs: by TMA, or
                 // 16 lanes a row, zeros past the last row (rows past it are never stored).
-                if (n > 0) {
-                    for (int g = 0; g < groups && ok; ++g) {
-                        if (asked[g] > 0 && !wait_long(kBarQFree + g, asked[g] - 1)) {
-                            ok = false;
-                            break;
-                        }
-                        ++asked[g];
-                        if (a.q_map) {  // two boxes: the heads of 128 / group tokens are the rows in order
-                            if (lane == 0) {
-                                tc::mbar_arrive_expect_tx(bar(kBarQ + g), kOperand);
-                                const int32_t token = u.first + (u.row0 + g * kGroupRows) / a.group;
-                                for (int slab = 0; slab < 2; ++slab)
-                                    tma_load_4d(base + kOffQ + g * kOperand + slab * kSlab, &maps.q, 64 * slab, z * a.group, token,
-                                                a.starts ? 0 : u.seq, bar(kBarQ + g));
-                            }
-                            continue;
-                        }
-                        const int c = lane & 15, row0 = g * kGroupRows + (lane >> 4);
-                        RowWalk at(a, z, u.row0 + row0, 2);
-                        const T* q = static_cast<const T*>(a.q) + u.seq * a.q_seq + u.first * a.q_token + c * 8;
-                        const uint32_t to = base + kOffQ + g * kOperand + (c >> 3) * kSlab;
-#pragma unroll 8
-                        for (int i = 0; i < kGroupRows; i += 2, at.next()) {
-                            const int row = i + (lane >> 4);
-                            const bool valid = row0 + i < rows;
-                            tc::cp_async_16_zfill(to + row * 128 + (((c ^ row) & 7) << 4),
-                                                  valid ? q + at.head * a.q_head + at.token * a.q_token : q, valid);
-                        }
-                        cp_async_commit();
+                for (int g = 0; g < groups; ++g) {
+                    if (asked[g] > 0 && !wait_long(kBarQFree + g, asked[g] - 1)) return false;
+                    ++asked[g];
+                    if (a.q_map) {  // two boxes: the heads of 128 / group tokens are the rows in order
+                        if (lane == 0) tc::mbar_arrive_expect_tx(bar(kBarQ + g), kOperand);
+                        __syncwarp();
+                        const int32_t token = u.first + (u.row0 + g * kGroupRows) / a.group;
+                        for (int slab = 0; slab < 2; ++slab)
+                            tma_load_4d_elect(base + kOffQ + g * kOperand + slab * kSlab, &maps.q, 64 * slab, z * a.group, token,
+                                              a.starts ? 0 : u.seq, bar(kBarQ + g));
+                        continue;
                     }
-                    if (!a.q_map) {
-                        if (ok && groups == 2) {
-                            cp_async_wait<1>();
-                            tc::fence_proxy_async_smem();
-                            __syncwarp();
-                            if (lane == 0) tc::mbar_arrive(bar(kBarQ));
-                        }
-                        cp_async_wait<0>();
+                    const int c = lane & 15, row0 = g * kGroupRows + (lane >> 4);
+                    RowWalk at(a, z, u.row0 + row0, 2);
+                    const T* q = static_cast<const T*>(a.q) + u.seq * a.q_seq + u.first * a.q_token + c * 8;
+                    const uint32_t to = base + kOffQ + g * kOperand + (c >> 3) * kSlab;
+#pragma unroll 8
+                    for (int i = 0; i < kGroupRows; i += 2, at.next()) {
+                        const int row = i + (lane >> 4);
+                        const bool valid = row0 + i < rows;
+                        tc::cp_async_16_zfill(to + row * 128 + (((c ^ row) & 7) << 4),
+                                              valid ? q + at.head * a.q_head + at.token * a.q_token : q, valid);
+                    }
+                    cp_async_commit();
+                }
+                if (!a.q_map) {
+                    if (groups == 2) {
+                        cp_async_wait<1>();
                         tc::fence_proxy_async_smem();
                         __syncwarp();
-                        if (ok && lane == 0) tc::mbar_arrive(bar(kBarQ + groups - 1));
+                        if (lane == 0) tc::mbar_arrive(bar(kBarQ));
                     }
+                    cp_async_wait<0>();
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(bar(kBarQ + groups - 1));
                 }
-                // The next job is asked for shortly before this one's end, not sooner: a place taken early would wait
-                // behind this job while other SMs run dry.
-                if (!ok || (n > 0 && !wait_long(kBarAsk, asked[0] - 1))) break;
+                return true;
+            };
+            // Job j + 1, asked for shortly before job j's end, not sooner: a place taken early would wait behind that
+            // job while other SMs run dry.
+            auto ask = [&](int j) {
+                if (now > 0 && !wait_long(kBarAsk, asked[0] - 1)) return false;
                 if (lane == 0) {
                     tc::mbar_arrive_expect_tx(bar(kBarNext), 16);
                     ask_next(base + kOffNext, bar(kBarNext));
                 }
-                if (!tc::mbar_wait_suspend(bar(kBarNext), j & 1, abort_flag, kWaitLimit, /*honor_abort=*/false)) ok = false;
+                bool ok = tc::mbar_wait_suspend(bar(kBarNext), j & 1, abort_flag, kWaitLimit, /*honor_abort=*/false);
                 ok = __all_sync(0xffffffffu, ok);
                 const bool more = read_next(base + kOffNext, x, y, z);
                 tc::fence_proxy_async_smem();
                 __syncwarp();
-                if (ok && !more) {
-                    if (j >= 1 && !wait_long(kBarJobFree + ((j + 1) & 1), ((j + 1) >> 1) - 1)) break;
-                    if (lane == 0) {
-                        jobs[(j + 1) & 1].n = -1;
-                        tc::mbar_arrive(bar(kBarJob + ((j + 1) & 1)));
-                    }
-                    break;
+                if (!ok) return false;
+                if (more) return publish(j + 1);
+                if (j >= 1 && !wait_long(kBarJobFree + ((j + 1) & 1), ((j + 1) >> 1) - 1)) return false;
+                if (lane == 0) {
+                    jobs[(j + 1) & 1].n = -1;
+                    tc::mbar_arrive(bar(kBarJob + ((j + 1) & 1)));
                 }
-            }
-            // Queries that were asked for have landed before the CTA ends.
-            for (int g = 0; g < kGroups; ++g)
-                if (a.q_map && lane == 0 && asked[g] > 0)
-                    tc::mbar_wait_suspend(bar(kBarQ + g), (asked[g] - 1) & 1, abort_flag, kWaitLimit, /*honor_abort=*/false);
-            __syncwarp();
-        } else if (warp == kLoadWarp) {
-            // ---- loader: K and V tiles in the order of use, one box a lane ----
-            const int boxes = kKeys / box_rows;  // of a 64-column slab
-            int ring = 0;
-            bool ok = true;
-            for (int j = 0; ok; ++j) {
-                if (!job_ready(j)) break;
-                const Job& job = jobs[j & 1];
-                const int n = job.n;
-                if (n < 0) break;
-                const ChunkUnit u = job.u;
-                const KeyTiles t = job.t;
-                const int begin = job.begin, kvh = job.kvh;
-                auto key = [&](int i) {
-                    const bool is_v = i == 2 * n - 1 || (i > 0 && (i & 1) == 0);
-                    const int tile = i == 0 ? 0 : i == 2 * n - 1 ? n - 1 : is_v ? i / 2 - 1 : (i + 1) / 2;
-                    return t.tile(begin + tile) * kKeys + (lane >> 1) * box_rows;
-                };
-                auto page_of = [&](int i) { return i < 2 * n && lane < 2 * boxes ? chunk_page(a, u, t, key(i), box_rows) : 0; };
-                int32_t page = page_of(0);
-                for (int i = 0; i < 2 * n; ++i, ++ring) {
-                    const int st = ring % kStages, use = ring / kStages;
-                    const bool is_v = i == 2 * n - 1 || (i > 0 && (i & 1) == 0);
-                    const int32_t next = page_of(i + 1);  // looked up while this tile waits for its place
-                    if (use > 0 && !wait(kBarEmpty + st, use - 1)) {
-                        ok = false;
-                        break;
-                    }
-                    if (lane == 0) tc::mbar_arrive_expect_tx(bar(kBarFull + st), kOperand);
-                    __syncwarp();
-                    if (lane < 2 * boxes)
-                        tma_load_4d(base + kOffRing + st * kOperand + (lane & 1) * kSlab + (lane >> 1) * box_rows * 128,
-                                    is_v ? &maps.v : &maps.k, 64 * (lane & 1), chunk_page_row(a, key(i)), kvh, page,
-                                    bar(kBarFull + st));
-                    page = next;
-                    __syncwarp();
-                }
-                done_with(j);
-            }
-            if (lane == 0)  // every copy has landed before the CTA ends
-                for (int st = 0; st < kStages && st < ring; ++st)
-                    tc::mbar_wait_suspend(bar(kBarFull + st), ((ring - 1 - st) / kStages) & 1, abort_flag, kWaitLimit,
-                                          /*honor_abort=*/false);
-            __syncwarp();
-        } else if (warp >= kOutWarp) {
-            // ---- finished rows: o = O / l, lse = m * kappa + log2(l); a row that nothing reached gives zeros and
-            // -inf. A row is a lane; the softmax is at the next job meanwhile ----
+                return true;
+            };
+            // ---- all four: finished rows: o = O / l, lse = m * kappa + log2(l); a row that nothing reached gives
+            // zeros and -inf. A row is a lane; the softmax is at the next job meanwhile ----
             const int r = tid & 127;
             int tiles[kGroups] = {0, 0}, rounds[kGroups] = {0, 0};
-            bool ok = true;
+            bool ok = warp > kOutWarp || publish(0);
             for (int j = 0; ok; ++j) {
                 if (!job_ready(j)) break;
                 const Job& job = jobs[j & 1];
@@ -362,6 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 const int64_t seq = job.u.seq;
                 const int64_t part = job.split * a.rows_total + (a.starts ? first : seq * a.tokens) * a.heads;
                 done_with(j);
+                if (warp == kOutWarp && !ask(j)) break;
                 for (int g = 0; g * kGroupRows < rows; ++g) {
                     float mk = 0.f, l = 0.f;
                     if (n > 0) {
@@ -415,23 +416,26 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     }
                 }
             }
+            // Queries that were asked for have landed before the CTA ends.
+            for (int g = 0; g < kGroups; ++g)
+                if (a.q_map && lane == 0 && asked[g] > 0)
+                    tc::mbar_wait_suspend(bar(kBarQ + g), (asked[g] - 1) & 1, abort_flag, kWaitLimit, /*honor_abort=*/false);
             __syncwarp();
         } else {
             // ---- products of group g: S(t + 1) as soon as S(t) is in registers, then O += P(t) V(t) ----
             const int g = warp - kMmaWarp;
             const uint64_t qdesc = tc::smem_desc(base + kOffQ + g * kOperand, 16, 1024, tc::kSwizzle128B);
             const uint64_t pdesc = tc::smem_desc(base + kOffP + g * kOperand, 16, 1024, tc::kSwizzle128B);
-            int ring = 0, tiles = 0, rounds = 0;
-            auto full = [&](int item) { return wait(kBarFull + item % kStages, item / kStages); };
-            auto issue_s = [&](int item) {
-                const uint64_t kdesc = tc::smem_desc(base + kOffRing + (item % kStages) * kOperand, 16, 1024, tc::kSwizzle128B);
+            int keys = 0, tiles = 0, rounds = 0;
+            const uint64_t kdesc = tc::smem_desc(base + kOffK, 16, 1024, tc::kSwizzle128B);
+            auto issue_s = [&]() {
 #pragma unroll
                 for (int s = 0; s < 8; ++s) {  // 16 dims a step: 32 bytes on inside a 64-column slab
                     const uint32_t off = ((s >> 2) * kSlab + (s & 3) * 32) >> 4;
                     tc::mma_ss_elect(tmem + col_s(g), qdesc + off, kdesc + off, idesc<T>(0), s > 0 ? 1u : 0u);
                 }
                 tc::mma_commit_elect(bar(kBarS + g));
-                tc::mma_commit_elect(bar(kBarEmpty + item % kStages));
+                tc::mma_commit_elect(bar(kBarKFree));
             };
             bool ok = true, early = false;  // early: S(0) of the job is on its way
             for (int j = 0; ok; ++j) {
@@ -441,11 +445,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 done_with(j);
                 if (n == 0) continue;
                 if (g >= groups) {  // the tiles of the other group alone
-                    for (int i = 0; i < 2 * n && ok; ++i) {
-                        ok = full(ring + i);
-                        if (ok && lane == 0) tc::mbar_arrive(bar(kBarEmpty + (ring + i) % kStages));
+                    for (int i = 0; i < n && ok; ++i, ++keys) {
+                        ok = wait(kBarK, keys);
+                        if (ok && lane == 0) tc::mbar_arrive(bar(kBarKFree));
+                        ok = ok && wait(kBarV + keys % kVStages, keys / kVStages);
+                        if (ok && lane == 0) tc::mbar_arrive(bar(kBarVFree + keys % kVStages));
                     }
-                    ring += 2 * n;
                     continue;
                 }
                 for (int i = early ? 0 : -1; i < n; ++i) {
@@ -457,46 +462,44 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                         early = false;
                         if (there(kBarJob + ((j + 1) & 1), (j + 1) >> 1)) {
                             const int n2 = jobs[(j + 1) & 1].n, groups2 = jobs[(j + 1) & 1].rows > kGroupRows ? 2 : 1;
-                            const int next = ring + 2 * n;
-                            if (n2 > 0 && g < groups2 && there(kBarQ + g, rounds + 1) &&
-                                there(kBarFull + next % kStages, next / kStages)) {
+                            if (n2 > 0 && g < groups2 && there(kBarQ + g, rounds + 1) && there(kBarK, keys + n)) {
                                 if (!wait(kBarSFree + g, tiles + i)) {
                                     ok = false;
                                     break;
                                 }
                                 tc::fence_after_sync();
-                                issue_s(next);
+                                issue_s();
                                 if (n2 == 1) tc::mma_commit_elect(bar(kBarQFree + g));
                                 early = true;
                             }
                         }
                     } else {
-                        if ((i < 0 && !wait(kBarQ + g, rounds)) || !full(ring + item_k(i + 1)) ||
+                        if ((i < 0 && !wait(kBarQ + g, rounds)) || !wait(kBarK, keys + i + 1) ||
                             (tiles + i >= 0 && !wait(kBarSFree + g, tiles + i))) {
                             ok = false;
                             break;
                         }
                         tc::fence_after_sync();
-                        issue_s(ring + item_k(i + 1));
+                        issue_s();
                         if (i + 2 == n) tc::mma_commit_elect(bar(kBarQFree + g));
                     }
                     if (i < 0) continue;
-                    const int item = ring + item_v(i, n);
-                    if (!full(item) || (i == 0 && rounds > 0 && !wait(kBarOFree + g, rounds - 1)) || !wait(kBarP + g, tiles + i)) {
+                    const int st = (keys + i) % kVStages;
+                    if (!wait(kBarV + st, (keys + i) / kVStages) || (i == 0 && rounds > 0 && !wait(kBarOFree + g, rounds - 1)) || !wait(kBarP + g, tiles + i)) {
                         ok = false;
                         break;
                     }
                     tc::fence_after_sync();
                     const uint64_t vdesc =
-                        tc::smem_desc(base + kOffRing + (item % kStages) * kOperand, kSlab, 1024, tc::kSwizzle128B);
+                        tc::smem_desc(base + kOffV + st * kOperand, kSlab, 1024, tc::kSwizzle128B);
 #pragma unroll
                     for (int s = 0; s < 8; ++s)  // 16 keys a step; V rows as they lie (MN-major)
                         tc::mma_ss_elect(tmem + col_o(g), pdesc + (((s >> 2) * kSlab + (s & 3) * 32) >> 4),
                                          vdesc + ((s * 16 * 128) >> 4), idesc<T>(1), (i > 0 || s > 0) ? 1u : 0u);
                     tc::mma_commit_elect(bar(kBarO + g));
-                    tc::mma_commit_elect(bar(kBarEmpty + item % kStages));
+                    tc::mma_commit_elect(bar(kBarVFree + st));
                 }
-                ring += 2 * n;
+                keys += n;
                 tiles += n;
                 ++rounds;
             }
@@ -510,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
         const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t s_col = lane_base + col_s(g), o_col = lane_base + col_o(g);
         const uint32_t p_row = base + kOffP + g * kOperand + r * 128;
-        int ring = 0, tiles = 0, turns = 0, rounds = 0;
+        int keys = 0, tiles = 0, turns = 0, rounds = 0;
         bool ok = true;
         for (int j = 0; ok; ++j) {
             if (!job_ready(j)) break;
@@ -521,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             const int g_row0 = job.u.row0 + g * kGroupRows;
             const int g_rows = min(kGroupRows, job.rows - g * kGroupRows);
             if (g_rows <= 0 || n == 0) {  // the group has no rows, or nothing to do for them
-                ring += 2 * n;
+                keys += n;
                 done_with(j);
                 continue;
             }
@@ -671,13 +674,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 // groups clear them, each before its own product.
                 const KeyTiles& t = job.t;
                 if (partly && (!t.any(k0) || !t.any(k0 + kKeys - 1) || (k0 < t.first.low && k0 + kKeys > t.last.sink))) {
-                    const int item = ring + item_v(i, n);
-                    if (!wait(kBarFull + item % kStages, item / kStages)) {
+                    const int st = (keys + i) % kVStages;
+                    if (!wait(kBarV + st, (keys + i) / kVStages)) {
                         ok = false;
                         break;
                     }
                     if (!t.any(k0 + r)) {
-                        const uint32_t v_row = base + kOffRing + (item % kStages) * kOperand + r * 128;
+                        const uint32_t v_row = base + kOffV + st * kOperand + r * 128;
 #pragma unroll
                         for (int c = 0; c < 16; ++c)  // in an order without bank conflicts
                             store_shared(v_row + (c >> 3) * kSlab + (((c ^ r) & 7) << 4), 0, 0, 0, 0);
@@ -691,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             if (!ok || (rounds > 0 && !wait(kBarOFree + g, rounds - 1))) break;
             *reinterpret_cast<float2*>(mem + kOffSums + (g * kGroupRows + r) * 8) = make_float2(mk, l);
             tc::mbar_arrive(bar(kBarSum + g));
-            ring += 2 * n;
+            keys += n;
             tiles += n;
             if (groups == 2) turns += n;
             ++rounds;
