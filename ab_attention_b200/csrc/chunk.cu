@@ -12,18 +12,98 @@ constexpr int kClusterUpTo = 16;
 // Waves of CTAs for ragged sequences: 48 of up to 16,000 keys take 277 / 266 / 265 / 268 / 282 us with
 // 4 / 6 / 8 / 12 / 20, and 292 us with clusters of 7 equal parts (a cluster waits for its slowest CTA).
 constexpr int kRaggedWaves = 8;
-constexpr int kRaggedJobs = 5;
+// Jobs an SM for ragged chunks on the tile kernel, if all were as long as the table allows: nine of 30 to 701 tokens
+// over up to 8,000 keys take 188 / 188 / 195 / 195 us with 2 / 3 / 4 / 5, and 211 us unsplit.
+constexpr int kRaggedJobs = 3;
 
-// Joins the splits of each row: o = sum_s 2^(lse_s - lse) o_s. kWarps warps a row, four dims a lane;
-// reads splits * 516 bytes a row. Launched while the splits still run: it waits for them here.
-template <class T, int kWarps>
+// Joins the splits of each row: o = sum_s 2^(lse_s - lse) o_s. A block a row, four dims a lane, each warp an
+// eighth of the splits; reads splits * 516 bytes a row.
+template <class T>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
-    __shared__ float4 part[8][32];
-    __shared__ float2 stat[8];
+    constexpr int kWarps = 8;
+    __shared__ float4 part[kWarps][32];
+    __shared__ float2 stat[kWarps];
     cudaGridDependencySynchronize();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int w = warp % kWarps;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (8 / kWarps) + warp / kWarps;
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row = blockIdx.x;
+    const int64_t token = row / a.heads;
+    const int head = static_cast<int>(row - token * a.heads);
+    int64_t seq = 0, at = token;
+    if (a.starts == nullptr) {
+        seq = token / a.tokens;
+        at = token - seq * a.tokens;
+    } else if (token < __ldg(a.starts) || token >= __ldg(a.starts + a.seqs)) {
+        return;  // in no sequence: left as it was
+    }
+    if (a.span > 0 && a.part_lse[row] == kWhole) return;  // written by its only split
+    // This warp's splits w, w + 8, ..: 32 at a time, their sums' weights against a running maximum.
+    float top = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int base = w; base < a.splits; base += 32 * kWarps) {
+        const int s = base + lane * kWarps;
+        const float x = s < a.splits ? a.part_lse[s * a.rows_total + row] : -INFINITY;
+        float next = x;
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, d));
+        next = fmaxf(next, top);
+        if (next == -INFINITY && !__any_sync(0xffffffffu, isnan(x))) continue;
+        const float scale = next == top ? 1.f : exp2f(top - next), f = exp2f(x - next);  // a NaN stays one
+        top = next;
+        sum = sum * scale + f;
+        acc.x *= scale, acc.y *= scale, acc.z *= scale, acc.w *= scale;
+        const int count = min(32, (a.splits - base + kWarps - 1) / kWarps);
+#pragma unroll 4
+        for (int i = 0; i < count; ++i) {
+            const float4 v = *reinterpret_cast<const float4*>(
+                a.part_o + (static_cast<int64_t>(base + i * kWarps) * a.rows_total + row) * 128 + 4 * lane);
+            const float fi = __shfl_sync(0xffffffffu, f, i);
+            acc.x += fi * v.x;
+            acc.y += fi * v.y;
+            acc.z += fi * v.z;
+            acc.w += fi * v.w;
+        }
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    part[w][lane] = acc;
+    if (lane == 0) stat[w] = make_float2(top, sum);
+    __syncthreads();
+    if (w != 0) return;
+    top = -INFINITY;
+    bool reached = false;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+        top = fmaxf(top, stat[i].x);
+        reached |= stat[i].y != 0.f;
+    }
+    sum = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (reached) {
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            const float f = exp2f(stat[i].x - top);
+            const float4 v = part[i][lane];
+            sum += f * stat[i].y;
+            acc.x += f * v.x;
+            acc.y += f * v.y;
+            acc.z += f * v.z;
+            acc.w += f * v.w;
+        }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const uint2 pair = make_uint2(Pair<T>::pack(acc.x * inv, acc.y * inv), Pair<T>::pack(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + seq * a.o_seq + head * a.o_head + at * a.o_token + 4 * lane) = pair;
+    if (a.lse != nullptr && lane == 0)
+        a.lse[seq * a.l_seq + head * a.l_head + at * a.l_token] = sum == 0.f ? -INFINITY : top + log2f(sum);
+}
+
+// The same for many rows: eight lanes a row, 16 dims a lane, so that a warp has four rows in flight and all loads of
+// a row's splits (eight at a time) go out together.
+template <class T>
+__global__ void __launch_bounds__(256) chunk_join_rows_kernel(const ChunkArgs a) {
+    cudaGridDependencySynchronize();
+    const int lane = threadIdx.x & 7;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 3);
     const int64_t token = row / a.heads;
     const int head = static_cast<int>(row - token * a.heads);
     int64_t seq = 0, at = token;
@@ -35,76 +115,54 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
         mine = mine && token >= __ldg(a.starts) && token < __ldg(a.starts + a.seqs);  // else left as it was
     }
     if (mine && a.span > 0) mine = a.part_lse[row] != kWhole;  // written by its only split
-    // This warp's splits w, w + kWarps, ..: 32 at a time, their sums' weights against a running maximum.
+    const unsigned lanes = 0xffu << (threadIdx.x & 24);
+    if (!mine) return;  // whole groups of eight lanes
     float top = -INFINITY, sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (mine) {
-        for (int base = w; base < a.splits; base += 32 * kWarps) {
-            const int s = base + lane * kWarps;
-            const float x = s < a.splits ? a.part_lse[s * a.rows_total + row] : -INFINITY;
-            float next = x;
+    float4 acc[4] = {};
+    for (int base = 0; base < a.splits; base += 8) {
+        const float x = base + lane < a.splits ? a.part_lse[static_cast<int64_t>(base + lane) * a.rows_total + row] : -INFINITY;
+        float next = x;
 #pragma unroll
-            for (int d = 16; d > 0; d /= 2) next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, d));
-            next = fmaxf(next, top);
-            if (next == -INFINITY && !__any_sync(0xffffffffu, isnan(x))) continue;
-            const float scale = next == top ? 1.f : exp2f(top - next), f = exp2f(x - next);  // a NaN stays one
-            top = next;
-            sum = sum * scale + f;
-            acc.x *= scale, acc.y *= scale, acc.z *= scale, acc.w *= scale;
-            const int count = min(32, (a.splits - base + kWarps - 1) / kWarps);
+        for (int d = 4; d > 0; d /= 2) next = fmaxf(next, __shfl_xor_sync(lanes, next, d));
+        next = fmaxf(next, top);
+        if (next == -INFINITY && !__any_sync(lanes, isnan(x))) continue;
+        const float scale = next == top ? 1.f : exp2f(top - next), f = exp2f(x - next);  // a NaN stays one
+        top = next;
+        sum = sum * scale + f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k].x *= scale, acc[k].y *= scale, acc[k].z *= scale, acc[k].w *= scale;
+        const int count = min(8, a.splits - base);
 #pragma unroll 4
-            for (int i = 0; i < count; ++i) {
-                const float4 v = *reinterpret_cast<const float4*>(
-                    a.part_o + (static_cast<int64_t>(base + i * kWarps) * a.rows_total + row) * 128 + 4 * lane);
-                const float fi = __shfl_sync(0xffffffffu, f, i);
-                acc.x += fi * v.x;
-                acc.y += fi * v.y;
-                acc.z += fi * v.z;
-                acc.w += fi * v.w;
+        for (int i = 0; i < count; ++i) {
+            const float4* from =
+                reinterpret_cast<const float4*>(a.part_o + (static_cast<int64_t>(base + i) * a.rows_total + row) * 128) + lane;
+            const float fi = __shfl_sync(lanes, f, i, 8);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float4 v = from[8 * k];
+                acc[k].x += fi * v.x;
+                acc[k].y += fi * v.y;
+                acc[k].z += fi * v.z;
+                acc[k].w += fi * v.w;
             }
         }
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     }
-    if constexpr (kWarps > 1) {
-        part[warp][lane] = acc;
-        if (lane == 0) stat[warp] = make_float2(top, sum);
-        __syncthreads();
-        if (w != 0) return;
-        float all = -INFINITY;
-        bool reached = false;
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i) {
-            all = fmaxf(all, stat[warp + i].x);
-            reached |= stat[warp + i].y != 0.f;
-        }
-        sum = 0.f;
-        acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (reached) {
-#pragma unroll
-            for (int i = 0; i < kWarps; ++i) {
-                const float f = exp2f(stat[warp + i].x - all);
-                const float4 v = part[warp + i][lane];
-                sum += f * stat[warp + i].y;
-                acc.x += f * v.x;
-                acc.y += f * v.y;
-                acc.z += f * v.z;
-                acc.w += f * v.w;
-            }
-        }
-        top = all;
-    }
-    if (!mine) return;
+    for (int d = 4; d > 0; d /= 2) sum += __shfl_xor_sync(lanes, sum, d);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const uint2 pair = make_uint2(Pair<T>::pack(acc.x * inv, acc.y * inv), Pair<T>::pack(acc.z * inv, acc.w * inv));
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + seq * a.o_seq + head * a.o_head + at * a.o_token + 4 * lane) = pair;
+    T* out = static_cast<T*>(a.o) + seq * a.o_seq + head * a.o_head + at * a.o_token + 4 * lane;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<uint2*>(out + 32 * k) =
+            make_uint2(Pair<T>::pack(acc[k].x * inv, acc[k].y * inv), Pair<T>::pack(acc[k].z * inv, acc[k].w * inv));
     if (a.lse != nullptr && lane == 0)
         a.lse[seq * a.l_seq + head * a.l_head + at * a.l_token] = sum == 0.f ? -INFINITY : top + log2f(sum);
 }
 
-template <class T, int kWarps>
-cudaError_t launch_join(const ChunkArgs& a, cudaStream_t stream) {
-    const int64_t blocks = ceil_div(a.rows_total, 8 / kWarps);
+// The join starts while the last CTAs of the splits still run, and waits for them itself.
+template <class Kernel>
+cudaError_t launch_join(Kernel kernel, int rows, const ChunkArgs& a, cudaStream_t stream) {
+    const int64_t blocks = ceil_div(a.rows_total, rows);
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -115,7 +173,7 @@ cudaError_t launch_join(const ChunkArgs& a, cudaStream_t stream) {
     config.stream = stream;
     config.attrs = &early;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, chunk_join_kernel<T, kWarps>, a);
+    return cudaLaunchKernelEx(&config, kernel, a);
 }
 
 }  // namespace
@@ -192,8 +250,9 @@ cudaError_t launch_chunk(const ChunkArgs& a, const ChunkMaps& maps, bool fp16, i
 cudaError_t launch_chunk_join(const ChunkArgs& a, bool fp16, cudaStream_t stream) {
     // A block a row while there are few rows: the splits' loads are what a row waits for.
     if (a.rows_total <= 8 * kSms)
-        return fp16 ? launch_join<half, 8>(a, stream) : launch_join<bf16, 8>(a, stream);
-    return fp16 ? launch_join<half, 1>(a, stream) : launch_join<bf16, 1>(a, stream);
+        return fp16 ? launch_join(chunk_join_kernel<half>, 1, a, stream) : launch_join(chunk_join_kernel<bf16>, 1, a, stream);
+    return fp16 ? launch_join(chunk_join_rows_kernel<half>, 32, a, stream)
+                : launch_join(chunk_join_rows_kernel<bf16>, 32, a, stream);
 }
 
 }  // namespace abx

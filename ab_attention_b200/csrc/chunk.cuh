@@ -90,6 +90,7 @@ __device__ __forceinline__ ChunkUnit chunk_unit(const ChunkArgs& a, int u, int t
     }
     const int lane = threadIdx.x & 31;
     int before = 0;
+#pragma unroll 1
     for (int base = 0; base < a.seqs; base += 32) {
         const int s = base + lane;
         int32_t first = 0, n = 0, len = 0, tiles = 0;
@@ -165,10 +166,10 @@ struct KeyTiles {
 };
 
 template <int kKeys>
-__device__ __forceinline__ KeyTiles chunk_tiles(const ChunkArgs& a, const ChunkUnit& u, int row0, int row1) {
+__device__ __forceinline__ KeyTiles chunk_tiles(const Seen& first, const Seen& last) {
     KeyTiles t;
-    t.first = chunk_seen(a, u, row0);
-    t.last = chunk_seen(a, u, row1);
+    t.first = first;
+    t.last = last;
     const int32_t high = (t.last.end + kKeys - 1) / kKeys;
     t.low = min(t.first.low / kKeys, high);
     t.head = min((t.last.sink + kKeys - 1) / kKeys, t.low);
@@ -185,8 +186,9 @@ __device__ __forceinline__ bool chunk_part(const ChunkArgs& a, int count, int s,
         end = min(begin + a.span, count);
         return count <= a.span;
     } else {
-        begin = static_cast<int>(static_cast<int64_t>(count) * s / a.splits);
-        end = static_cast<int>(static_cast<int64_t>(count) * (s + 1) / a.splits);
+        const int each = count / a.splits, more = count - each * a.splits;  // the first `more` parts take one more
+        begin = each * s + min(s, more);
+        end = begin + each + (s < more);
         return a.splits == 1;
     }
 }

@@ -78,7 +78,8 @@ static_assert(kSmemBytes <= 227 * 1024, "shared memory exceeds the per-block lim
 constexpr uint32_t kTmemColumns = 512;
 __device__ __forceinline__ constexpr uint32_t col_o(int g) { return 128u * static_cast<uint32_t>(g); }
 __device__ __forceinline__ constexpr uint32_t col_s(int g) { return 256u + 128u * static_cast<uint32_t>(g); }
-constexpr uint64_t kWaitLimit = 400ull * 1000 * 1000;
+constexpr uint64_t kWaitLimit = 400ull * 1000 * 1000;  // cycles, of the waits at a CTA's end
+constexpr int kPolls = 1 << 22;
 constexpr float kGrow = 8.0f;               // log2
 constexpr float kLargeScore = 1048576.0f;   // log2: above, s * kappa - m * kappa is off by more than a few units
 
@@ -179,11 +180,28 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-    auto wait = [&](int b, int phase) { return tc::mbar_wait_warp_suspend(bar(b), phase & 1, abort_flag, kWaitLimit); };
+    // Waits are bounded by their polls (each may suspend the warp for a while): the library's wait by the clock is
+    // four times the code, and at some 40 places it alone would fill a third of the instruction cache.
+    auto wait = [&](int b, int phase) {
+        if (__all_sync(0xffffffffu, tc::mbar_try_wait_suspend(bar(b), phase & 1))) return true;
+#pragma unroll 1
+        for (int spin = 0; spin < kPolls; ++spin) {
+            if (__all_sync(0xffffffffu, tc::mbar_try_wait_suspend(bar(b), phase & 1))) return true;
+            if ((spin & 15) == 15 && *abort_flag) break;
+        }
+        *abort_flag = 1;
+        return false;
+    };
     auto there = [&](int b, int phase) { return __all_sync(0xffffffffu, tc::mbar_try_wait(bar(b), phase & 1)) != 0; };
     // For waits of a tile's length and more: the warp sleeps through them and leaves the issue slots alone.
     auto wait_long = [&](int b, int phase) {
-        return tc::mbar_wait_warp(bar(b), phase & 1, abort_flag, kWaitLimit, tc::kLongWaitHintNs);
+#pragma unroll 1
+        for (int spin = 0; spin < kPolls; ++spin) {
+            if (__all_sync(0xffffffffu, tc::mbar_try_wait(bar(b), phase & 1, tc::kLongWaitHintNs))) return true;
+            if (*abort_flag) break;
+        }
+        *abort_flag = 1;
+        return false;
     };
     // The j-th job's slot, once it is written; done_with() gives it back (once a warp).
     auto job_ready = [&](int j) { return wait_long(kBarJob + (j & 1), j >> 1); };
@@ -202,6 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             const int boxes = kKeys / box_rows;  // of a 64-column slab
             int keys = 0;
             bool ok = true;
+#pragma unroll 1
             for (int j = 0; ok; ++j) {
                 if (!job_ready(j)) break;
                 const Job& job = jobs[j & 1];
@@ -219,6 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     row = boxes > 1 ? 0 : chunk_page_row(a, k0);
                 };
                 if (n > 0) look_up(0);
+#pragma unroll 1
                 for (int i = 0; i < n; ++i, ++keys) {
                     const int st = is_v ? keys % kVStages : 0, use = is_v ? keys / kVStages : keys;
                     if (use > 0 && !wait((is_v ? kBarVFree : kBarKFree) + st, use - 1)) {
@@ -228,6 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     const uint32_t to = base + (is_v ? kOffV : kOffK) + st * kOperand, full = bar((is_v ? kBarV : kBarK) + st);
                     if (lane == 0) tc::mbar_arrive_expect_tx(full, kOperand);
                     __syncwarp();
+#pragma unroll 1
                     for (int b = 0; b < boxes; ++b) {
                         const int32_t p = __shfl_sync(0xffffffffu, page, b);
                         tma_load_4d_elect(to + b * box_rows * 128, map, 0, row, kvh, p, full);
@@ -247,45 +268,58 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             __syncwarp();
         } else if (warp >= kOutWarp) {
             // ---- the first of them: jobs. This CTA's own place in the grid, then the places of CTAs that have not
-            // started. Tiles of rows fastest, then splits, then key heads: CTAs that run at the same time share K and
-            // V in L2 ----
+            // started. Tiles of rows fastest, then key heads, then splits: CTAs that run at the same time share K and V
+            // in L2, and the last parts of ragged sequences, short or empty, come last ----
             int x = blockIdx.x, y = blockIdx.y, z = blockIdx.z;
             int asked[kGroups] = {0, 0};  // rounds of queries
-            int now = 0;                  // key tiles of the latest job
+            int questions = 0;
+            ChunkUnit u;                  // the latest job
+            KeyTiles t;
+            Seen bound{};                 // of the row that this lane stands for
+            int rows = 0, begin = 0, n = 0;
+            bool whole = false;
+            auto work_out = [&]() {
+                u = chunk_unit(a, x, kGroups * kGroupRows);
+                rows = u.seq < 0 ? 0 : min(kGroups * kGroupRows, u.n * a.group - u.row0);
+                n = begin = 0;
+                whole = false;
+                if (rows <= 0) return;
+                // A lane for each row that matters: the tile's first and last, the groups' first and last.
+                const int which = lane < 2 ? (lane == 0 ? 0 : rows - 1)
+                                           : (lane & 2 ? (lane & 1) * kGroupRows : min(((lane & 1) + 1) * kGroupRows, rows) - 1);
+                bound = chunk_seen(a, u, u.row0 + min(which, rows - 1));
+                auto of = [&](int from) {
+                    return Seen{__shfl_sync(0xffffffffu, bound.sink, from), __shfl_sync(0xffffffffu, bound.low, from),
+                                __shfl_sync(0xffffffffu, bound.end, from)};
+                };
+                t = chunk_tiles<kKeys>(of(0), of(1));
+                int end;
+                whole = chunk_part(a, t.count, z, begin, end);
+                n = end - begin;
+                if (whole && z > 0) rows = n = 0;  // nothing to do
+            };
             auto publish = [&](int j) {
-                const ChunkUnit u = chunk_unit(a, x, kGroups * kGroupRows);
-                int rows = u.seq < 0 ? 0 : min(kGroups * kGroupRows, u.n * a.group - u.row0);
-                KeyTiles t{};
-                int begin = 0, end = 0;
-                bool whole = false;
-                if (rows > 0) {
-                    t = chunk_tiles<kKeys>(a, u, u.row0, u.row0 + rows - 1);
-                    whole = chunk_part(a, t.count, y, begin, end);
-                    if (whole && y > 0) rows = 0;  // nothing to do
-                }
-                const int n = rows > 0 ? end - begin : 0, groups = rows > kGroupRows ? 2 : 1;
-                now = n;
+                const int groups = rows > kGroupRows ? 2 : 1;
                 if (j >= 2 && !wait_long(kBarJobFree + (j & 1), (j >> 1) - 1)) return false;
                 Job& job = jobs[j & 1];
                 if (lane == 0) {
                     job.u = u;
                     job.t = t;
-                    job.kvh = z;
-                    job.split = y;
+                    job.kvh = y;
+                    job.split = z;
                     job.rows = rows;
                     job.whole = whole;
                     job.begin = begin;
                     job.n = n;
                 }
-                if (lane < groups && rows > 0) {
-                    job.low[lane] = chunk_seen(a, u, u.row0 + lane * kGroupRows);
-                    job.high[lane] = chunk_seen(a, u, u.row0 + min((lane + 1) * kGroupRows, rows) - 1);
-                }
+                if (lane >= 2 && lane < 4) job.low[lane & 1] = bound;
+                if (lane >= 4 && lane < 6) job.high[lane & 1] = bound;
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(bar(kBarJob + (j & 1)));
                 if (n == 0) return true;
                 // The rows' queries, as soon as the last scores of the job before are done with theirs: by TMA, or
                 // 16 lanes a row, zeros past the last row (rows past it are never stored).
+#pragma unroll 1
                 for (int g = 0; g < groups; ++g) {
                     if (asked[g] > 0 && !wait_long(kBarQFree + g, asked[g] - 1)) return false;
                     ++asked[g];
@@ -293,16 +327,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                         if (lane == 0) tc::mbar_arrive_expect_tx(bar(kBarQ + g), kOperand);
                         __syncwarp();
                         const int32_t token = u.first + (u.row0 + g * kGroupRows) / a.group;
+#pragma unroll 1
                         for (int slab = 0; slab < 2; ++slab)
-                            tma_load_4d_elect(base + kOffQ + g * kOperand + slab * kSlab, &maps.q, 64 * slab, z * a.group, token,
+                            tma_load_4d_elect(base + kOffQ + g * kOperand + slab * kSlab, &maps.q, 64 * slab, y * a.group, token,
                                               a.starts ? 0 : u.seq, bar(kBarQ + g));
                         continue;
                     }
                     const int c = lane & 15, row0 = g * kGroupRows + (lane >> 4);
-                    RowWalk at(a, z, u.row0 + row0, 2);
+                    RowWalk at(a, y, u.row0 + row0, 2);
                     const T* q = static_cast<const T*>(a.q) + u.seq * a.q_seq + u.first * a.q_token + c * 8;
                     const uint32_t to = base + kOffQ + g * kOperand + (c >> 3) * kSlab;
-#pragma unroll 8
+#pragma unroll 2
                     for (int i = 0; i < kGroupRows; i += 2, at.next()) {
                         const int row = i + (lane >> 4);
                         const bool valid = row0 + i < rows;
@@ -325,25 +360,34 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 }
                 return true;
             };
-            // Job j + 1, asked for shortly before job j's end, not sooner: a place taken early would wait behind that
-            // job while other SMs run dry.
-            auto ask = [&](int j) {
-                if (now > 0 && !wait_long(kBarAsk, asked[0] - 1)) return false;
-                if (lane == 0) {
-                    tc::mbar_arrive_expect_tx(bar(kBarNext), 16);
-                    ask_next(base + kOffNext, bar(kBarNext));
+            // Job j: the CTA's own place, then one asked for shortly before the end of the job before it, not sooner: a
+            // place taken early would wait behind that job while other SMs run dry.
+            auto find = [&](int j) {
+                if (n > 0 && !wait_long(kBarAsk, asked[0] - 1)) return false;
+                bool more = true, own = j == 0;
+#pragma unroll 1
+                for (rows = 0; more && rows == 0; own = false) {  // places with nothing to do are passed over
+                    if (!own) {
+                        if (lane == 0) {
+                            tc::mbar_arrive_expect_tx(bar(kBarNext), 16);
+                            ask_next(base + kOffNext, bar(kBarNext));
+                        }
+                        bool ok =
+                            tc::mbar_wait_suspend(bar(kBarNext), questions & 1, abort_flag, kWaitLimit, /*honor_abort=*/false);
+                        ok = __all_sync(0xffffffffu, ok);
+                        ++questions;
+                        more = read_next(base + kOffNext, x, y, z);
+                        tc::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (!ok) return false;
+                    }
+                    if (more) work_out();
                 }
-                bool ok = tc::mbar_wait_suspend(bar(kBarNext), j & 1, abort_flag, kWaitLimit, /*honor_abort=*/false);
-                ok = __all_sync(0xffffffffu, ok);
-                const bool more = read_next(base + kOffNext, x, y, z);
-                tc::fence_proxy_async_smem();
-                __syncwarp();
-                if (!ok) return false;
-                if (more) return publish(j + 1);
-                if (j >= 1 && !wait_long(kBarJobFree + ((j + 1) & 1), ((j + 1) >> 1) - 1)) return false;
+                if (more) return publish(j);
+                if (j >= 2 && !wait_long(kBarJobFree + (j & 1), (j >> 1) - 1)) return false;
                 if (lane == 0) {
-                    jobs[(j + 1) & 1].n = -1;
-                    tc::mbar_arrive(bar(kBarJob + ((j + 1) & 1)));
+                    jobs[j & 1].n = -1;
+                    tc::mbar_arrive(bar(kBarJob + (j & 1)));
                 }
                 return true;
             };
@@ -351,18 +395,24 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             // zeros and -inf. A row is a lane; the softmax is at the next job meanwhile ----
             const int r = tid & 127;
             int tiles[kGroups] = {0, 0}, rounds[kGroups] = {0, 0};
-            bool ok = warp > kOutWarp || publish(0);
-            for (int j = 0; ok; ++j) {
-                if (!job_ready(j)) break;
-                const Job& job = jobs[j & 1];
-                const int n = job.n, rows = job.rows;
-                const bool whole = job.whole != 0;
-                if (n < 0) break;
-                const int32_t first = job.u.first, kvh = job.kvh, row0 = job.u.row0;
-                const int64_t seq = job.u.seq;
-                const int64_t part = job.split * a.rows_total + (a.starts ? first : seq * a.tokens) * a.heads;
-                done_with(j);
-                if (warp == kOutWarp && !ask(j)) break;
+            bool ok = true;
+#pragma unroll 1
+            for (int j = -1; ok; ++j) {
+                int n = 0, rows = 0;
+                bool whole = false;
+                int32_t first = 0, kvh = 0, row0 = 0;
+                int64_t seq = 0, part = 0;
+                if (j >= 0) {
+                    if (!job_ready(j)) break;
+                    const Job& job = jobs[j & 1];
+                    n = job.n, rows = job.rows, whole = job.whole != 0;
+                    if (n < 0) break;
+                    first = job.u.first, kvh = job.kvh, row0 = job.u.row0, seq = job.u.seq;
+                    part = job.split * a.rows_total + (a.starts ? first : seq * a.tokens) * a.heads;
+                    done_with(j);
+                }
+                if (warp == kOutWarp && !find(j + 1)) break;
+#pragma unroll 1
                 for (int g = 0; g * kGroupRows < rows; ++g) {
                     float mk = 0.f, l = 0.f;
                     if (n > 0) {
@@ -438,6 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 tc::mma_commit_elect(bar(kBarKFree));
             };
             bool ok = true, early = false;  // early: S(0) of the job is on its way
+#pragma unroll 1
             for (int j = 0; ok; ++j) {
                 if (!job_ready(j)) break;
                 const int n = jobs[j & 1].n, groups = jobs[j & 1].rows > kGroupRows ? 2 : 1;
@@ -445,6 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 done_with(j);
                 if (n == 0) continue;
                 if (g >= groups) {  // the tiles of the other group alone
+#pragma unroll 1
                     for (int i = 0; i < n && ok; ++i, ++keys) {
                         ok = wait(kBarK, keys);
                         if (ok && lane == 0) tc::mbar_arrive(bar(kBarKFree));
@@ -453,6 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     }
                     continue;
                 }
+#pragma unroll 1
                 for (int i = early ? 0 : -1; i < n; ++i) {
                     if (g == 0 && lane == 0 && i == max(n - kAskAhead, 0)) tc::mbar_arrive(bar(kBarAsk));
                     __syncwarp();
@@ -515,6 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
         const uint32_t p_row = base + kOffP + g * kOperand + r * 128;
         int keys = 0, tiles = 0, turns = 0, rounds = 0;
         bool ok = true;
+#pragma unroll 1
         for (int j = 0; ok; ++j) {
             if (!job_ready(j)) break;
             const Job& job = jobs[j & 1];
@@ -535,6 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             float m = -INFINITY;   // the row's reference, a bare score
             float mk = 0.f;        // m * kappa, 0 while m is -inf
             float l = 0.f;
+#pragma unroll 1
             for (int i = 0; i < n; ++i) {
                 const int32_t k0 = (begin + i < head ? begin + i : low + begin + i) * kKeys;
                 if (!wait(kBarS + g, tiles + i)) {
@@ -722,7 +777,7 @@ cudaError_t launch(const ChunkArgs& a, const ChunkMaps& maps, int box_rows, cuda
     if (attr.numRegs * kThreads < 8 * 32 * kSoftmaxRegs + (kThreads - 8 * 32) * kOtherRegs) return cudaErrorInvalidConfiguration;
     const int64_t units = chunk_units(a);
     if (units > 0x7fffffff || a.splits > 65535) return cudaErrorInvalidConfiguration;
-    kernel<<<dim3(static_cast<unsigned>(units), a.splits, a.kv_heads), kThreads, kSmemBytes, stream>>>(a, maps, box_rows);
+    kernel<<<dim3(static_cast<unsigned>(units), a.kv_heads, a.splits), kThreads, kSmemBytes, stream>>>(a, maps, box_rows);
     return cudaGetLastError();
 }
 

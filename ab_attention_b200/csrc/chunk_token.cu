@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
     const ChunkUnit u = chunk_unit(a, blockIdx.z, L::rows);
     if (u.seq < 0) return;  // past the last tile
     const int rows = min(L::rows, u.n * a.group - u.row0);
-    const KeyTiles t = chunk_tiles<kKeys>(a, u, u.row0, u.row0 + rows - 1);
+    const KeyTiles t = chunk_tiles<kKeys>(chunk_seen(a, u, u.row0), chunk_seen(a, u, u.row0 + rows - 1));
     int begin, end;
     const bool whole = chunk_part(a, t.count, split, begin, end);
     if (whole && split > 0) return;
