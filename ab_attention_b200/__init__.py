@@ -6,8 +6,8 @@ from .layout import cube_layout
 from .rotary import RotaryAxes, apply_rotary, grid_positions
 
 __all__ = ["SamplePlan", "ab_attention", "apply_plan", "build_plan", "dense_attention", "dense_cross_attention",
-           "paged_attention", "cube_layout", "VideoAttention", "hunyuan_attention", "ab_attention_host",
+           "paged_attention", "cube_layout", "VideoAttention", "hunyuan_attention", "StreamAttention", "ab_attention_host",
            "window_attention", "KVCache", "kv_cache", "append_kv", "chunk_attention", "RotaryAxes", "apply_rotary",
            "grid_positions"]
-from .video import VideoAttention, hunyuan_attention  # noqa: E402
+from .video import StreamAttention, VideoAttention, hunyuan_attention  # noqa: E402
 from .pipeline import ab_attention_host  # noqa: E402

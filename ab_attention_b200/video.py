@@ -13,6 +13,8 @@ from __future__ import annotations
 import torch
 
 from .attention import SamplePlan, apply_plan, build_plan, dense_attention, dense_cross_attention
+from .cache import append_kv, chunk_attention, kv_cache
+from .rotary import VIDEO_AXES, grid_positions
 
 
 def plan_seed(layer: int, anchor: int) -> int:
@@ -108,3 +110,81 @@ def hunyuan_attention(schedule, layer, q, k, v, video_tokens, prompt_tokens):
         outputs.append(dense_cross_attention(sl(q, prompt_end, q.shape[2]), None, None,
                                              extra_kv=(sl(k, prompt_end, q.shape[2]), sl(v, prompt_end, q.shape[2]))))
     return torch.cat(outputs, dim=2)
+
+
+class StreamAttention:
+    """Attention of a video that is generated chunk by chunk (no counterpart in the reference).
+
+    A chunk is ``chunk_frames`` latent frames of ``height`` x ``width`` tokens. Its queries attend to
+    the chunk itself in both directions and to the frames before it: to all of them, or to the last
+    ``window_frames`` (the chunk's own counted) and the first ``sink_frames``. Keys and values
+    live in a paged cache per layer, turned by their (frame, row, column) positions; with a
+    window, pages behind it are used again, so the cache does not grow with the video.
+
+    Call the object once per layer and denoising step of a chunk (each call replaces the chunk's keys and
+    values), then ``advance()`` once the chunk is final. Nothing synchronises: ``advance`` updates device
+    counters in place, so a captured step replays for chunk after chunk.
+    """
+
+    def __init__(self, heads, height, width, *, max_frames, kv_heads=None, chunk_frames=1, window_frames=None, sink_frames=0,
+                 batch=1, axes=VIDEO_AXES, page_size=128, dtype=torch.bfloat16, device="cuda"):
+        if min(heads, height, width, chunk_frames, batch) < 1 or max_frames < chunk_frames:
+            raise ValueError("heads, height, width, chunk_frames and batch must be positive, max_frames at least chunk_frames")
+        if window_frames is not None and window_frames < chunk_frames:
+            raise ValueError("window_frames must be at least chunk_frames: a chunk attends to itself")
+        if sink_frames < 0:
+            raise ValueError("sink_frames must not be negative")
+        frame = height * width
+        self.heads, self.kv_heads, self.batch, self.axes = heads, kv_heads or heads, batch, axes
+        self.max_frames, self.chunk_frames, self.tokens = max_frames, chunk_frames, chunk_frames * frame
+        self.window = None if window_frames is None else window_frames * frame
+        self.sinks = sink_frames * frame
+        # Logical pages of a sequence, and the places they take: the sinks' own, then a ring that holds the window,
+        # the chunk and the pages cut by their ends.
+        logical = -(-max_frames * frame // page_size)
+        places = logical
+        if self.window is not None:
+            kept = -(-self.sinks // page_size)
+            places = min(logical, kept + -(-(self.window + self.tokens) // page_size) + 2)
+        page = torch.arange(logical, dtype=torch.int32)
+        if places < logical:
+            page = torch.where(page < kept, page, kept + (page - kept) % (places - kept))
+        table = page + places * torch.arange(batch, dtype=torch.int32)[:, None]
+        self.page_table = table.to(torch.int32).contiguous().to(device)
+        self.starts = torch.arange(batch + 1, dtype=torch.int32, device=device) * self.tokens
+        self.lengths = torch.empty(batch, dtype=torch.int32, device=device)
+        self.positions = torch.empty(batch * self.tokens, 3, dtype=torch.int32, device=device)
+        self._first = grid_positions(chunk_frames, height, width, device=device).repeat(batch, 1)
+        self._cache = dict(pages=places * batch, kv_heads=self.kv_heads, page_size=page_size, dtype=dtype, device=device)
+        self.caches = {}
+        self.reset()
+
+    def reset(self):
+        """The next chunk is the first."""
+        self.frames = 0
+        self.lengths.fill_(self.tokens)
+        self.positions.copy_(self._first)
+
+    def advance(self):
+        """The current chunk is final; the next one follows it."""
+        if self.frames + 2 * self.chunk_frames > self.max_frames:
+            raise ValueError(f"the stream holds {self.max_frames} frames")
+        self.frames += self.chunk_frames
+        self.lengths.add_(self.tokens)
+        self.positions[:, 0].add_(self.chunk_frames)
+
+    @torch.no_grad()
+    def __call__(self, layer, q, k, v):
+        """q [B,H,N,128], k and v [B,Hk,N,128] of the chunk's N tokens (before rotation), any strides with
+        contiguous rows; returns [B,H,N,128], a view of token-major [B,N,H,128] memory."""
+        if q.shape != (self.batch, self.heads, self.tokens, 128):
+            raise ValueError(f"q must be {[self.batch, self.heads, self.tokens, 128]} (got {list(q.shape)})")
+        if k.shape != (self.batch, self.kv_heads, self.tokens, 128) or v.shape != k.shape:
+            raise ValueError(f"k and v must be {[self.batch, self.kv_heads, self.tokens, 128]}")
+        if layer not in self.caches:
+            self.caches[layer] = kv_cache(**self._cache)
+        cache, where = self.caches[layer], (self.page_table, self.starts, self.lengths)
+        q, k, v = (x.transpose(1, 2).flatten(0, 1) for x in (q, k, v))  # packed; a view for one batch
+        q = append_kv(cache, k, v, *where, positions=self.positions, axes=self.axes, q=q)
+        out = chunk_attention(q, cache, *where, longest=self.tokens, window=self.window, sinks=self.sinks, block=self.tokens)
+        return out.unflatten(0, (self.batch, self.tokens)).transpose(1, 2)

@@ -548,3 +548,62 @@ def test_frames_of_a_stream_equal_one_pass():
     hold(whole[0].transpose(0, 1), lse[0].T, *rows, v, window=2 * block, sinks=10, block=block)
     hold(torch.cat(outs), None, *rows, v, window=2 * block, sinks=10, block=block)
     assert torch.equal(stream.rows_of(cache.keys, table[0], n), rows[1])
+
+
+@pytest.mark.parametrize("batch,heads,kv,chunk,window,sinks,page,frames", [
+    (1, 4, 4, 1, None, 0, 16, 5), (2, 6, 2, 2, 4, 1, 32, 12), (1, 2, 1, 1, 2, 2, 64, 9), (1, 3, 3, 3, 3, 0, 128, 9),
+])
+def test_stream_attention(batch, heads, kv, chunk, window, sinks, page, frames):
+    """Chunk after chunk, two layers, two denoising steps each, pages used again behind the window: the last
+    step's outputs are those of one pass over the whole video."""
+    h, w, layers = 6, 11, 2
+    frame, g = h * w, gen(frames)
+    s = ab.StreamAttention(heads, h, w, kv_heads=kv, chunk_frames=chunk, window_frames=window, sink_frames=sinks, batch=batch,
+                           max_frames=frames, page_size=page)
+    q, k, v = (normal(g, layers, batch, x, frames * frame, 128) for x in (heads, kv, kv))
+    with pytest.raises(ValueError, match="q must be"):
+        s(0, q[0], k[0], v[0])
+    for turn in range(2):  # a second video after reset()
+        outs = [[] for _ in range(layers)]
+        for f in range(0, frames, chunk):
+            rows = slice(f * frame, (f + chunk) * frame)
+            for layer in range(layers):
+                s(layer, q[layer, :, :, rows] * 0.5, k[layer, :, :, rows] * 2, v[layer, :, :, rows] - 1)  # a noisier step
+                outs[layer].append(s(layer, *(x[layer, :, :, rows] for x in (q, k, v))))
+            if f + chunk < frames:
+                s.advance()
+        with pytest.raises(ValueError, match="holds"):
+            s.advance()
+        s.reset()
+        p = ab.grid_positions(frames, h, w, device="cuda")
+        for layer in range(layers):
+            tq, tk = ab.apply_rotary(q[layer], k[layer], p)
+            got = torch.cat(outs[layer], 2)
+            for b in range(batch):
+                hold(got[b].transpose(0, 1), None, tq[b].transpose(0, 1), tk[b].transpose(0, 1), v[layer, b].transpose(0, 1),
+                     window=None if window is None else window * frame, sinks=sinks * frame, block=chunk * frame)
+    if window is not None:
+        assert s.caches[0].keys.shape[0] <= batch * (-(-(window + chunk + sinks) * frame // page) + 3)
+
+
+def test_stream_attention_in_a_graph():
+    """A captured step serves chunk after chunk: advance() moves its counters on."""
+    g = gen(3)
+    s = ab.StreamAttention(2, 5, 9, max_frames=6, window_frames=3)
+    q, k, v = (normal(g, 1, 2, 45, 128) for _ in range(3))
+    want = []
+    for f in range(6):
+        q.copy_(normal(gen(f), 1, 2, 45, 128)), k.copy_(normal(gen(f + 50), 1, 2, 45, 128))
+        want.append(s(0, q, k, v).clone())
+        if f < 5:
+            s.advance()
+    s.reset()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = s(0, q, k, v)
+    for f in range(6):
+        q.copy_(normal(gen(f), 1, 2, 45, 128)), k.copy_(normal(gen(f + 50), 1, 2, 45, 128))
+        graph.replay()
+        assert torch.equal(out, want[f])
+        if f < 5:
+            s.advance()

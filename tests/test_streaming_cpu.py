@@ -246,3 +246,19 @@ def test_restated_turn_back_is_the_gradient():
     grad = torch.autograd.grad((f(x) * g[0]).sum(), x)[0][0]
     back = stream.turn(g[:1], p[:1], (64, 64), 50.0, inverse=True)[0]
     assert torch.allclose(grad, back)
+
+
+def test_stream_attention_places():
+    """Logical pages of a stream take distinct places while any of them is in the window."""
+    s = ab.StreamAttention(2, 6, 11, kv_heads=1, chunk_frames=2, window_frames=4, sink_frames=1, batch=2, max_frames=40,
+                           page_size=16, device="cpu")
+    frame, table = 66, s.page_table
+    assert table.shape == (2, -(-40 * 66 // 16)) and not set(table[0].tolist()) & set(table[1].tolist())
+    for f in range(0, 40, 2):
+        end = (f + 2) * frame
+        keys = list(range(frame)) + list(range(max(0, end - 4 * frame), end))
+        pages = sorted({x // 16 for x in keys})
+        assert len({table[0, x].item() for x in pages}) == len(pages)
+    for bad in (dict(window_frames=1), dict(sink_frames=-1), dict(max_frames=1), dict(batch=0)):
+        with pytest.raises(ValueError):
+            ab.StreamAttention(2, 6, 11, **{**dict(chunk_frames=2, max_frames=8, device="cpu"), **bad})
