@@ -246,7 +246,7 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
 
 // All threads of all CTAs of the cluster; what they wrote before is seen after.
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
 }
 // This CTA's shared address `at`, read in CTA `rank` of the cluster.
 __device__ __forceinline__ float cluster_load(uint32_t at, int rank) {

@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
     volatile int* abort_flag = reinterpret_cast<volatile int*>(mem + L::abort_flag);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = blockIdx.x, kvh = blockIdx.y;
-    const ChunkUnit u = chunk_unit(a, blockIdx.z, L::rows);
+    const int split = blockIdx.z, kvh = blockIdx.y;
+    const ChunkUnit u = chunk_unit(a, blockIdx.x, L::rows);
     if (u.seq < 0) return;  // past the last tile
     const int rows = min(L::rows, u.n * a.group - u.row0);
     const KeyTiles t = chunk_tiles<kKeys>(chunk_seen(a, u, u.row0), chunk_seen(a, u, u.row0 + rows - 1));
@@ -410,13 +410,13 @@ cudaError_t launch(const ChunkArgs& a, const ChunkMaps& maps, int box_rows, cuda
     cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L::bytes));
     if (err != cudaSuccess) return err;
     const int64_t units = chunk_units(a);
-    if (units > 65535 || a.splits > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    if (units > 0x7fffffff || a.splits > 65535) return cudaErrorInvalidConfiguration;
     cudaLaunchAttribute cluster{};
     cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = a.cluster ? a.splits : 1;
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cluster.val.clusterDim.x = cluster.val.clusterDim.y = 1;
+    cluster.val.clusterDim.z = a.cluster ? a.splits : 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(a.splits, a.kv_heads, static_cast<unsigned>(units));
+    config.gridDim = dim3(static_cast<unsigned>(units), a.kv_heads, a.splits);
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = L::bytes;
     config.stream = stream;

@@ -393,6 +393,108 @@ def test_bad_pages_lengths_and_chunks_are_reported(new):
         assert torch.equal(ab.chunk_attention(b.q, b.cache, *b.plan, longest=new), good)
 
 
+@pytest.mark.parametrize("new", [1, 90])
+def test_joint_buffers_and_strided_outputs(new):
+    """Keys and values in one buffer, outputs head by head, queries whose heads repeat: as contiguous tensors."""
+    b = Batch(14, [(new, 700), (new, 90)], 4, 2, 32, BF)
+    want, want_lse = ab.chunk_attention(b.q, b.cache, *b.plan, longest=new, return_lse=True)
+    joint = torch.stack((b.keys, b.values), 1)
+    out = torch.empty(4, 2 * new, 128, dtype=BF, device="cuda").transpose(0, 1)
+    got, lse = ab.chunk_attention(b.q, ab.KVCache(joint[:, 0], joint[:, 1]), *b.plan, longest=new, return_lse=True, out=out)
+    assert got is out and torch.equal(got, want) and torch.equal(lse, want_lse)
+    one = b.q[:, :1].expand(-1, 4, -1)
+    assert torch.equal(ab.chunk_attention(one, b.cache, *b.plan, longest=new),
+                       ab.chunk_attention(one.contiguous(), b.cache, *b.plan, longest=new))
+
+
+@pytest.mark.parametrize("heads,kv,tokens,keys", [(256, 1, 3, 300), (96, 1, 9, 200), (34, 2, 40, 333), (130, 1, 1, 50)])
+def test_wide_groups(heads, kv, tokens, keys):
+    """Many query heads on one key head, in groups that do and do not divide a tile of rows."""
+    g = gen(heads)
+    q, k, v = normal(g, 1, heads, tokens, 128), normal(g, 1, kv, keys, 128), normal(g, 1, kv, keys, 128)
+    o, lse = ab.window_attention(q, k, v, window=100, sinks=2, return_lse=True)
+    hold(o[0].transpose(0, 1), lse[0].T, *(x[0].transpose(0, 1) for x in (q, k, v)), window=100, sinks=2)
+
+
+def test_many_sequences():
+    """More sequences than a grid's second and third dim hold."""
+    g, n = gen(15), 70001
+    q, k, v = normal(g, n, 1, 1, 128), normal(g, n, 1, 3, 128), normal(g, n, 1, 3, 128)
+    o = ab.window_attention(q, k, v)
+    s = (q.float() @ k.float().transpose(-1, -2) * 128 ** -0.5).softmax(-1)
+    ref, a = s @ v.float(), s @ v.float().abs()
+    assert ((o.float() - ref).abs() <= (2 ** -8 * 1.01 + 5e-4) * a + 2 ** -8 * 1.01 * ref.abs()).all()
+
+
+def test_cache_past_32_bits():
+    """Pages whose elements lie past 2^31: stored and read where they belong."""
+    pages, kv, page, n = 132000, 1, 128, 300
+    keys = torch.empty(pages, kv, page, 128, dtype=BF, device="cuda")
+    values = torch.empty_like(keys)
+    assert keys.numel() > 2 ** 31
+    g = gen(16)
+    table = torch.tensor([[pages - 1, 5, pages - 3]], dtype=torch.int32, device="cuda")
+    starts, lengths = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, n], [n]))
+    k, v, q = normal(g, n, kv, 128), normal(g, n, kv, 128), normal(g, n, 2, 128)
+    cache = ab.KVCache(keys, values)
+    ab.append_kv(cache, k, v, table, starts, lengths)
+    assert torch.equal(keys[pages - 1, 0], k[:128, 0]) and torch.equal(values[pages - 3, 0, :44], v[256:, 0])
+    o, lse = ab.chunk_attention(q, cache, table, starts, lengths, return_lse=True)
+    hold(o, lse, q, k, v)
+    one = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    o, lse = ab.chunk_attention(q[-1:], cache, table, one, lengths, longest=1, return_lse=True)
+    hold(o, lse, q[-1:], k, v)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on the GPU have workspaces of their own."""
+    batches = [Batch(20 + i, [(1, 6000), (1, 900), (200, 700)], 4, 2, 16, BF) for i in range(2)]
+    want = [ab.chunk_attention(b.q, b.cache, *b.plan) for b in batches]
+    few = [ab.chunk_attention(b.q[:2], b.cache, b.table[:2], b.starts[:3], b.lengths[:2], longest=1) for b in batches]
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (b, stream) in enumerate(zip(batches, streams)):
+            with torch.cuda.stream(stream):
+                got[i].append((ab.chunk_attention(b.q, b.cache, *b.plan),
+                               ab.chunk_attention(b.q[:2], b.cache, b.table[:2], b.starts[:3], b.lengths[:2], longest=1)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) and torch.equal(y, few[i]) for x, y in got[i])
+
+
+def test_first_call_of_a_process_in_a_capture():
+    """A process whose first calls are captured (nothing warmed up) replays them."""
+    import subprocess
+    import sys
+
+    code = """
+import torch, ab_attention_b200 as ab
+x = torch.randn(1, 2, 300, 128, device="cuda").bfloat16(); y = x[:, :, :1].contiguous(); p = torch.zeros(300, 3, dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    outs = ab.window_attention(x, x, x), ab.window_attention(y, x, x), ab.apply_rotary(x, x, p)[0]
+x.normal_(); y.copy_(x[:, :, -1:]); p.fill_(7)
+g.replay()
+want = ab.window_attention(x, x, x), ab.window_attention(y, x, x), ab.apply_rotary(x, x, p)[0]
+assert all(torch.equal(a, b) for a, b in zip(outs, want))
+print("replayed")
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert "replayed" in run.stdout, run.stderr[-2000:]
+
+
+def test_inference_mode():
+    b = Batch(17, [(2, 50)], 2, 2, 16, BF)
+    want = ab.chunk_attention(b.q, b.cache, *b.plan)
+    with torch.inference_mode():
+        cache = ab.KVCache(b.keys.clone(), b.values.clone())
+        assert torch.equal(ab.chunk_attention(b.q.clone(), cache, *b.plan), want)
+        assert ab.append_kv(cache, b.k[0][:2], b.v[0][:2], *b.plan) is None
+
+
 def test_chunk_attention_of_nothing():
     b = Batch(7, [(0, 30), (0, 0)], 4, 2, 16, BF)
     assert ab.chunk_attention(b.q, b.cache, *b.plan).shape == (0, 4, 128)
