@@ -77,10 +77,13 @@ def chunk_attention(q, cache, page_table, starts, lengths, *, longest=None, wind
     _on_gpu(q)
     if window is not None and window < 1:
         raise ValueError("window must be positive, or None")
+    if longest is None:
+        longest = q.shape[0]
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    torch.ops.ab_attention.chunk_attention(q, cache.keys, cache.values, page_table, starts, lengths,
-                                           q.shape[0] if longest is None else longest, window or 0, sinks, block, out,
-                                           lse)
+        out, lse = torch.ops.ab_attention.chunk_attention(q, cache.keys, cache.values, page_table, starts, lengths, longest,
+                                                          window or 0, sinks, block, return_lse)
+    else:
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+        torch.ops.ab_attention.chunk_attention_out(q, cache.keys, cache.values, page_table, starts, lengths, longest,
+                                                   window or 0, sinks, block, out, lse)
     return (out, lse) if return_lse else out

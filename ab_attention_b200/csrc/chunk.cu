@@ -12,6 +12,9 @@ constexpr int kClusterUpTo = 16;
 // Waves of CTAs for ragged sequences: 48 of up to 16,000 keys take 277 / 266 / 265 / 268 / 282 us with
 // 4 / 6 / 8 / 12 / 20, and 292 us with clusters of 7 equal parts (a cluster waits for its slowest CTA).
 constexpr int kRaggedWaves = 8;
+// ... unless no part of the longest has more tiles than this without them: a part of 16 tiles takes 12 us, a join
+// with its launch 8 us more.
+constexpr int kRaggedTiles = 16;
 // Jobs an SM for ragged chunks on the tile kernel, if all were as long as the table allows: nine of 30 to 701 tokens
 // over up to 8,000 keys take 188 / 188 / 195 / 195 us with 2 / 3 / 4 / 5, and 211 us unsplit.
 constexpr int kRaggedJobs = 3;
@@ -187,7 +190,16 @@ int64_t chunk_units(const ChunkArgs& a) {
 
 void chunk_layout(ChunkArgs& a) {
     const int64_t rows = static_cast<int64_t>(a.longest) * a.group;
-    a.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 256;
+    a.tile_rows = rows <= 16 ? 16 : 32;
+    if (rows > 32) {
+        // More rows than one tile of the few-row kernel: it still is the faster one while all its CTAs run at once
+        // and have little to do (it starts in 6 us where the tile kernel takes 10). us of the few-row / the tile kernel,
+        // by 64-key steps: 8 heads on 2, 100 tokens on 100 keys 9.9 / 13.2 (52 steps), 200 on 200 12.0 / 14.8
+        // (200), 100 on 2,000 16.7 / 20.5 (832), 40 on 8,000 24.8 / 20.9 (1,250); 12 heads, 100 on 2,000 36 / 19 (1,536).
+        const int64_t ctas = chunk_units(a) * a.kv_heads;
+        const int64_t steps = ctas * ceil_div(a.keys, kChunkTokenKeys) / (a.starts != nullptr && a.seqs > 1 ? 2 : 1);
+        if (ctas > kSms || steps > 5 * kSms) a.tile_rows = 256;
+    }
     const int tile_keys = chunk_tile_keys(a);
     const int64_t ctas = chunk_units(a) * a.kv_heads;
     // Keys that one row tile can see, in tiles; the lengths themselves are known on the device only.
@@ -198,22 +210,25 @@ void chunk_layout(ChunkArgs& a) {
     }
     const int64_t tiles = ceil_div(keys, tile_keys);
     if (a.tile_rows < 256) {
-        // CTAs that fit the GPU at a time, and how many the call should come to: one wave where all sequences
-        // have one length, several where they are ragged (as if all were as long as the table allows: the
-        // lengths are on the device), so that they still balance. No part under four tiles.
+        // CTAs that fit the GPU at a time, and the parts of a row tile's keys that one wave of them has room for; no
+        // part under four tiles.
         const int64_t slots = kSms * (a.tile_rows == 16 ? 2 : 1);
         const bool ragged = a.starts != nullptr && a.seqs > 1;
-        const int64_t most = ceil_div(tiles, 4), want = ragged ? ceil_div(slots * kRaggedWaves, ctas) : slots / ctas;
-        int64_t splits = want < 1 ? 1 : want > most ? most : want;
+        const int64_t most = ceil_div(tiles, 4), room = slots / ctas < most ? slots / ctas : most;
+        const int64_t joined = room < kMaxCluster ? room : kMaxCluster;
         a.span = 0;
-        if (ragged) {  // equal spans, joined through the workspace
-            a.span = static_cast<int32_t>(ceil_div(tiles, splits));
-            splits = ceil_div(tiles, a.span);
-        } else if (splits < kClusterUpTo) {  // equal parts, joined in a cluster
-            splits = splits < kMaxCluster ? splits : kMaxCluster;
-            a.cluster = splits > 1;
+        if (room < kClusterUpTo && (!ragged || ceil_div(tiles, joined < 1 ? 1 : joined) <= kRaggedTiles)) {
+            a.splits = static_cast<int32_t>(joined < 1 ? 1 : joined);  // equal parts, joined in a cluster
+            a.cluster = a.splits > 1;
+        } else if (!ragged) {
+            a.splits = static_cast<int32_t>(room);  // few and long: equal parts, joined through the workspace
+        } else {
+            // Ragged and long: equal spans, joined through the workspace, that come to several waves if all sequences
+            // were as long as the table allows (the lengths are on the device), so that they still balance.
+            const int64_t want = ceil_div(slots * kRaggedWaves, ctas), parts = want > most ? most : want;
+            a.span = static_cast<int32_t>(ceil_div(tiles, parts));
+            a.splits = static_cast<int32_t>(ceil_div(tiles, a.span));
         }
-        a.splits = static_cast<int32_t>(splits);
         return;
     }
     // Equal parts, as many as make the waves of CTAs (one an SM) shortest: a part costs its tiles and

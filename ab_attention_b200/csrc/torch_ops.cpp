@@ -408,7 +408,7 @@ void check_chunk(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& 
     }
 }
 
-void chunk_attention_cuda(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values,
+void chunk_attention_out_cuda(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values,
                           const at::Tensor& page_table, const at::Tensor& starts, const at::Tensor& lengths,
                           int64_t longest, int64_t window, int64_t sinks, int64_t block, at::Tensor out,
                           std::optional<at::Tensor> lse) {
@@ -445,6 +445,22 @@ void chunk_attention_cuda(const at::Tensor& q, const at::Tensor& keys, const at:
     c.sinks = sinks;
     c.block = block;
     attend(c, q);
+}
+
+std::tuple<at::Tensor, at::Tensor> chunk_results(const at::Tensor& q, bool lse) {
+    TORCH_CHECK_VALUE(q.dim() == 3, "q must be [tokens, heads, 128] (got ", q.sizes(), ")");
+    return {at::empty(q.sizes(), q.options()),
+            lse ? at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat)) : at::Tensor()};
+}
+
+std::tuple<at::Tensor, at::Tensor> chunk_attention_cuda(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values,
+                                                        const at::Tensor& page_table, const at::Tensor& starts,
+                                                        const at::Tensor& lengths, int64_t longest, int64_t window,
+                                                        int64_t sinks, int64_t block, bool want_lse) {
+    auto [out, lse] = chunk_results(q, want_lse);
+    chunk_attention_out_cuda(q, keys, values, page_table, starts, lengths, longest, window, sinks, block, out,
+                             want_lse ? std::optional<at::Tensor>(lse) : std::nullopt);
+    return {out, want_lse ? lse : at::empty({0}, q.options().dtype(at::kFloat))};
 }
 
 void check_window(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t sinks, int64_t block) {
@@ -509,11 +525,21 @@ at::Tensor append_meta(at::Tensor keys, at::Tensor values, const at::Tensor& k, 
     return q ? at::empty(q->sizes(), q->options()) : at::empty({0}, keys.options());
 }
 
-void chunk_attention_meta(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values,
+void chunk_attention_out_meta(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values,
                           const at::Tensor& page_table, const at::Tensor& starts, const at::Tensor& lengths,
                           int64_t longest, int64_t window, int64_t sinks, int64_t block, at::Tensor out,
                           std::optional<at::Tensor> lse) {
     check_chunk(q, keys, values, page_table, starts, lengths, longest, window, sinks, block, out, lse);
+}
+
+std::tuple<at::Tensor, at::Tensor> chunk_attention_meta(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values,
+                                                        const at::Tensor& page_table, const at::Tensor& starts,
+                                                        const at::Tensor& lengths, int64_t longest, int64_t window,
+                                                        int64_t sinks, int64_t block, bool want_lse) {
+    auto [out, lse] = chunk_results(q, want_lse);
+    check_chunk(q, keys, values, page_table, starts, lengths, longest, window, sinks, block, out,
+                want_lse ? std::optional<at::Tensor>(lse) : std::nullopt);
+    return {out, want_lse ? lse : at::empty({0}, q.options().dtype(at::kFloat))};
 }
 
 std::tuple<at::Tensor, at::Tensor> window_attention_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
@@ -554,6 +580,8 @@ TORCH_LIBRARY(ab_attention, m) {
     m.def("append(Tensor(a!) keys, Tensor(b!) values, Tensor k, Tensor v, Tensor page_table, Tensor starts, "
           "Tensor lengths, Tensor? q, Tensor? positions, int[] sections, float theta, bool shared, bool halves) -> Tensor");
     m.def("chunk_attention(Tensor q, Tensor keys, Tensor values, Tensor page_table, Tensor starts, Tensor lengths, "
+          "int longest, int window, int sinks, int block, bool lse) -> (Tensor, Tensor)");
+    m.def("chunk_attention_out(Tensor q, Tensor keys, Tensor values, Tensor page_table, Tensor starts, Tensor lengths, "
           "int longest, int window, int sinks, int block, Tensor(a!) out, Tensor(b!)? lse) -> ()");
     m.def("window_attention(Tensor q, Tensor k, Tensor v, int window, int sinks, int block) -> (Tensor, Tensor)");
 }
@@ -566,6 +594,7 @@ TORCH_LIBRARY_IMPL(ab_attention, CUDA, m) {
     m.impl("rotary", &rotary_cuda);
     m.impl("append", &append_cuda);
     m.impl("chunk_attention", &chunk_attention_cuda);
+    m.impl("chunk_attention_out", &chunk_attention_out_cuda);
     m.impl("window_attention", &window_attention_cuda);
 }
 
@@ -577,12 +606,13 @@ TORCH_LIBRARY_IMPL(ab_attention, Meta, m) {
     m.impl("rotary", &rotary_meta);
     m.impl("append", &append_meta);
     m.impl("chunk_attention", &chunk_attention_meta);
+    m.impl("chunk_attention_out", &chunk_attention_out_meta);
     m.impl("window_attention", &window_attention_meta);
 }
 
 // No gradients, as everywhere in the package: the streaming operators pass the autograd keys by, which
 // also spares their callers a no_grad block.
 TORCH_LIBRARY_IMPL(ab_attention, Autograd, m) {
-    for (const char* name : {"rotary", "append", "chunk_attention", "window_attention"})
+    for (const char* name : {"rotary", "append", "chunk_attention", "chunk_attention_out", "window_attention"})
         m.impl(name, torch::CppFunction::makeFallthrough());
 }
