@@ -1,20 +1,38 @@
 // Many rows against many keys: attention of chunks of tokens on the tensor cores (tcgen05).
 //
-// One CTA takes 256 rows (two groups of 128, one TMEM lane and one softmax thread a
+// A CTA takes 256 rows (two groups of 128, one TMEM lane and one softmax thread a
 // row) of one key head and walks the 128-key tiles that any of them sees; K and V
 // tiles are read once for both groups. Per tile and group:
 //     S = Q K^T (TMEM, f32)  ->  P = 2^((s - m) * kappa) (registers, then shared memory, 16 bits)  ->  O += P V (TMEM, f32)
 // A softmax thread takes its whole S row into registers at once, which frees the S
 // columns: the product for the next tile runs while this tile's exponentials do,
 // because P goes to shared memory and not over S. A group's chain is then its
-// softmax alone, and the two groups share the tensor pipe and the exponential unit.
-// Bounds for a tile of both groups, in SM cycles: tensor pipe 2,048 (four products of
-// 128^3), exponential unit 2,048 (32,768 at 16 a cycle), shared memory 3,072 (operands
-// 2,048, P 512, incoming K and V 512).
+// softmax alone, about 3,240 cycles a tile: S read 150, maximum 360, exponentials
+// 1,550, stores and fence 120, and some 200 to 300 for each of three waits.
+//
+// The groups take turns at the exponentials. In phase, both groups' ran at half the
+// rate and the unit idled through the rest of the tile (3,850 cycles); in turns one
+// group's other steps fill the other's. Bounds for a tile of both groups, in SM
+// cycles: tensor pipe 2,048 (four products of 128^3), exponential unit 2,048 (32,768 at
+// 16 a cycle), shared memory 3,072 (operands 2,048, P 512, incoming K and V 512).
+// Measured for 3,600 rows x 12 heads over 75,600 keys (1,672 GFLOP): 1.43 ms alone
+// (1,170 TFLOP/s, tensor pipe and exponential unit 63% busy), 1.62 ms back to back,
+// where the GPU is at its power cap (993 W, 1.4 to 1.67 GHz) and fewer cycles no longer
+// shorten it.
+//
+// CTAs are persistent: near the end of its rows a CTA asks the grid's launch control for
+// the place of a CTA that has not started and goes on with that. Set-up and hand-over
+// between two tiles of rows otherwise cost 15,000 cycles (five tiles of keys): now the
+// next queries (TMA), keys and first scores arrive during the last tile, and four
+// warps of their own write finished rows during the next one. 8,191 tokens in a
+// window of 1,024 (ten tiles of keys each): 140 us with one CTA a tile of rows, 105 us so.
+// The code is kept small (100 KB; 159 KB cost 3 to 10%): a change of jobs runs code that
+// is not in the instruction cache.
 //
 // The maximum of a row is raised lazily (only when it grows by more than 2^8, so P stays
 // in fp16's range and O is rarely rescaled); sums and O are f32. P is rounded to the
-// element type for its product, as V is given in it; the row's sum takes P unrounded.
+// element type for its product, as V is given in it: half a unit of each weight, which
+// shows as an error of 1.4 times the result's own rounding. The row's sum takes P unrounded.
 #include "chunk.cuh"
 #include "f32x2.cuh"
 #include "tcgen05.cuh"
@@ -29,6 +47,8 @@ constexpr int kMmaWarp = 8;    // one warp a group
 constexpr int kLoadWarp = 10;  // one for K, one for V
 constexpr int kOutWarp = 12;   // four warps: finished rows; the first also finds the next job and loads its queries
 constexpr int kThreads = 16 * 32;
+// 512 threads start with 128 registers each. The split with no spills anywhere; 168/88, 184/72 and 192/64 measured
+// 1 to 2% slower.
 constexpr int kSoftmaxRegs = 176;
 constexpr int kOtherRegs = 80;
 constexpr int kAskAhead = 4;  // tiles before a job's end at which the next is asked for
