@@ -14,7 +14,7 @@
 // rate and the unit idled through the rest of the tile (3,850 cycles); in turns one
 // group's other steps fill the other's. Bounds for a tile of both groups, in SM
 // cycles: tensor pipe 2,048 (four products of 128^3), exponential unit 2,048 (32,768 at
-// 16 a cycle), shared memory 3,072 (operands 2,048, P 512, incoming K and V 512).
+// 16 a cycle), shared memory half as much again (operands 2,048, P 512, incoming K and V 512).
 // Measured for 3,600 rows x 12 heads over 75,600 keys (1,672 GFLOP): 1.43 ms alone
 // (1,170 TFLOP/s, tensor pipe and exponential unit 63% busy), 1.62 ms back to back,
 // where the GPU is at its power cap (993 W, 1.4 to 1.67 GHz) and fewer cycles no longer
@@ -115,6 +115,16 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+
+// One lane of a converged warp, always the same.
+__device__ __forceinline__ bool elected() {
+    uint32_t e;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+    return e != 0;
+}
+
+// A value that is the same in all lanes, so that the compiler may keep it in a uniform register.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 __device__ __forceinline__ void store_shared(uint32_t to, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(to), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -493,19 +503,23 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             __syncwarp();
         } else {
             // ---- products of group g: S(t + 1) as soon as S(t) is in registers, then O += P(t) V(t) ----
-            const int g = warp - kMmaWarp;
+            const int g = uniform(warp) - kMmaWarp;
+            const uint32_t tm = uniform(tmem);
             const uint64_t qdesc = tc::smem_desc(base + kOffQ + g * kOperand, 16, 1024, tc::kSwizzle128B);
             const uint64_t pdesc = tc::smem_desc(base + kOffP + g * kOperand, 16, 1024, tc::kSwizzle128B);
             int keys = 0, tiles = 0, rounds = 0;
             const uint64_t kdesc = tc::smem_desc(base + kOffK, 16, 1024, tc::kSwizzle128B);
             auto issue_s = [&]() {
+                if (elected()) {
 #pragma unroll
-                for (int s = 0; s < 8; ++s) {  // 16 dims a step: 32 bytes on inside a 64-column slab
-                    const uint32_t off = ((s >> 2) * kSlab + (s & 3) * 32) >> 4;
-                    tc::mma_ss_elect(tmem + col_s(g), qdesc + off, kdesc + off, idesc<T>(0), s > 0 ? 1u : 0u);
+                    for (int s = 0; s < 8; ++s) {  // 16 dims a step: 32 bytes on inside a 64-column slab
+                        const uint32_t off = ((s >> 2) * kSlab + (s & 3) * 32) >> 4;
+                        tc::mma_ss(tm + col_s(g), qdesc + off, kdesc + off, idesc<T>(0), s > 0 ? 1u : 0u);
+                    }
+                    tc::mma_commit(bar(kBarS + g));
+                    tc::mma_commit(bar(kBarKFree));
                 }
-                tc::mma_commit_elect(bar(kBarS + g));
-                tc::mma_commit_elect(bar(kBarKFree));
+                __syncwarp();
             };
             bool ok = true, early = false;  // early: S(0) of the job is on its way
 #pragma unroll 1
@@ -557,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                         if (i + 2 == n) tc::mma_commit_elect(bar(kBarQFree + g));
                     }
                     if (i < 0) continue;
-                    const int st = (keys + i) % kVStages;
+                    const int st = uniform((keys + i) % kVStages);
                     if (!wait(kBarV + st, (keys + i) / kVStages) || (i == 0 && rounds > 0 && !wait(kBarOFree + g, rounds - 1)) || !wait(kBarP + g, tiles + i)) {
                         ok = false;
                         break;
@@ -565,12 +579,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     tc::fence_after_sync();
                     const uint64_t vdesc =
                         tc::smem_desc(base + kOffV + st * kOperand, kSlab, 1024, tc::kSwizzle128B);
+                    if (elected()) {
 #pragma unroll
-                    for (int s = 0; s < 8; ++s)  // 16 keys a step; V rows as they lie (MN-major)
-                        tc::mma_ss_elect(tmem + col_o(g), pdesc + (((s >> 2) * kSlab + (s & 3) * 32) >> 4),
-                                         vdesc + ((s * 16 * 128) >> 4), idesc<T>(1), (i > 0 || s > 0) ? 1u : 0u);
-                    tc::mma_commit_elect(bar(kBarO + g));
-                    tc::mma_commit_elect(bar(kBarVFree + st));
+                        for (int s = 0; s < 8; ++s)  // 16 keys a step; V rows as they lie (MN-major)
+                            tc::mma_ss(tm + col_o(g), pdesc + (((s >> 2) * kSlab + (s & 3) * 32) >> 4), vdesc + ((s * 16 * 128) >> 4),
+                                       idesc<T>(1), (i > 0 || s > 0) ? 1u : 0u);
+                        tc::mma_commit(bar(kBarO + g));
+                        tc::mma_commit(bar(kBarVFree + st));
+                    }
+                    __syncwarp();
                 }
                 keys += n;
                 tiles += n;
