@@ -154,26 +154,32 @@ __device__ __forceinline__ Seen chunk_seen(const ChunkArgs& a, const ChunkUnit& 
     return s;
 }
 
-// The key tiles of rows [row0, row1]: [0, head) then [low, low + count - head).
+// The key tiles of a tile of rows: `head` of them from key 0 on (sinks), the others from key `base` on.
 struct KeyTiles {
-    int32_t head, low, count;
+    int32_t head, base, count;
     Seen first, last;  // of the first and the last row: every bound grows with the row
-    __device__ __forceinline__ int32_t tile(int i) const { return i < head ? i : low + (i - head); }
+    template <int kKeys>
+    __device__ __forceinline__ int32_t key(int i) const {
+        return i < head ? i * kKeys : base + (i - head) * kKeys;
+    }
     // Whether any row of the tile sees key j.
     __device__ __forceinline__ bool any(int32_t j) const {
         return j < last.end && (j >= first.low || j < last.sink);
     }
 };
 
+// Contiguous keys are walked from the first that is seen (a window's tiles are then one fewer on average); in
+// pages, tiles start where pages do.
 template <int kKeys>
-__device__ __forceinline__ KeyTiles chunk_tiles(const Seen& first, const Seen& last) {
+__device__ __forceinline__ KeyTiles chunk_tiles(const ChunkArgs& a, const Seen& first, const Seen& last) {
     KeyTiles t;
     t.first = first;
     t.last = last;
-    const int32_t high = (t.last.end + kKeys - 1) / kKeys;
-    t.low = min(t.first.low / kKeys, high);
-    t.head = min((t.last.sink + kKeys - 1) / kKeys, t.low);
-    t.count = t.head + high - t.low;
+    const int32_t low = min(first.low, last.end);
+    t.base = a.table == nullptr ? low : low / kKeys * kKeys;
+    t.head = (last.sink + kKeys - 1) / kKeys;
+    if (t.head * kKeys > t.base) t.head = t.base = 0;  // the sinks' tiles reach the window's: all from key 0
+    t.count = t.head + (last.end - t.base + kKeys - 1) / kKeys;
     return t;
 }
 

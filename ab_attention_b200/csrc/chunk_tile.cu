@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 done_with(j);
                 int32_t page = 0, row = 0;
                 auto look_up = [&](int i) {
-                    const int32_t k0 = t.tile(begin + i) * kKeys;
+                    const int32_t k0 = t.key<kKeys>(begin + i);
                     page = lane < boxes ? chunk_page(a, u, t, k0 + lane * box_rows, box_rows) : 0;
                     // a page of 128 keys and less is a box of its own and starts at its first row
                     row = boxes > 1 ? 0 : chunk_page_row(a, k0);
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     return Seen{__shfl_sync(0xffffffffu, bound.sink, from), __shfl_sync(0xffffffffu, bound.low, from),
                                 __shfl_sync(0xffffffffu, bound.end, from)};
                 };
-                t = chunk_tiles<kKeys>(of(0), of(1));
+                t = chunk_tiles<kKeys>(a, of(0), of(1));
                 int end;
                 whole = chunk_part(a, t.count, z, begin, end);
                 n = end - begin;
@@ -622,13 +622,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             const Seen mine = chunk_seen(a, job.u, g_row0 + min(r, g_rows - 1));
             // Tiles in [whole_low, whole_end) or below whole_sink are seen whole by all rows of the group.
             const int32_t whole_end = job.low[g].end, whole_low = job.high[g].low, whole_sink = job.low[g].sink;
-            const int32_t head = job.t.head, low = job.t.low - head, begin = job.begin;
+            const int32_t head = job.t.head, after = job.t.base - head * kKeys, begin = job.begin;
             float m = -INFINITY;   // the row's reference, a bare score
             float mk = 0.f;        // m * kappa, 0 while m is -inf
             float l = 0.f;
 #pragma unroll 1
             for (int i = 0; i < n; ++i) {
-                const int32_t k0 = (begin + i < head ? begin + i : low + begin + i) * kKeys;
+                const int32_t k0 = (begin + i) * kKeys + (begin + i < head ? 0 : after);
                 if (!wait(kBarS + g, tiles + i)) {
                     ok = false;
                     break;

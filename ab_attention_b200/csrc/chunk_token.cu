@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
     const ChunkUnit u = chunk_unit(a, blockIdx.x, L::rows);
     if (u.seq < 0) return;  // past the last tile
     const int rows = min(L::rows, u.n * a.group - u.row0);
-    const KeyTiles t = chunk_tiles<kKeys>(chunk_seen(a, u, u.row0), chunk_seen(a, u, u.row0 + rows - 1));
+    const KeyTiles t = chunk_tiles<kKeys>(a, chunk_seen(a, u, u.row0), chunk_seen(a, u, u.row0 + rows - 1));
     int begin, end;
     const bool whole = chunk_part(a, t.count, split, begin, end);
     if (whole && split > 0) return;
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
         const int boxes = kKeys / box_rows;  // of one slab
         const int op = lane / (2 * boxes), rest = lane % (2 * boxes), slab = rest & 1, box = rest >> 1;
         const uint32_t to = op * kOperand + slab * kSlab + box * box_rows * 128;
-        auto key = [&](int i) { return t.tile(begin + i) * kKeys + box * box_rows; };
+        auto key = [&](int i) { return t.key<kKeys>(begin + i) + box * box_rows; };
         int32_t page = lane < 4 * boxes && n > 0 ? chunk_page(a, u, t, key(0), box_rows) : 0;
         int issued = 0;
         for (int i = 0; i < n; ++i) {
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
             const int st = i % kStages;
             const uint32_t phase = (i / kStages) & 1;
             const uint32_t kbase = base + st * kStage, vbase = kbase + kOperand;
-            const int32_t k0 = t.tile(begin + i) * kKeys + warp * kWarpKeys;
+            const int32_t k0 = t.key<kKeys>(begin + i) + warp * kWarpKeys;
             if (!tc::mbar_wait_warp_suspend(k_full(st), phase, abort_flag, kWaitLimit)) break;
             // S = Q K^T for 16 keys (two 8-key column tiles), dims in eight steps of 16.
             float s[MT][2][4];
