@@ -15,14 +15,15 @@
 namespace abx {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kLanes = 8;                       // threads of a token
 constexpr int kGroups = kThreads / kLanes;
 // Heads in flight, blocks an SM and thread groups an SM, without and with a cache. Measured (us, one
-// B200): 75,600 tokens x 24 heads / 2 x 10,799 x 80 heads / 10,800 x 36 rows into pages: 152 / 146 / 43 for
-// (4, 2, 160), 155 / 156 / 39 for (2, 3, 64); a register limit that spills costs up to 2x.
+// B200): 75,600 tokens x 24 heads / 2 x 10,799 x 80 heads / 10,800 x 36 rows into pages: 150 / 142 / 45 for
+// (4, 4, 160), 155 / 156 / 39 for (2, 6, 64), 43 for (2, 6, 128) into pages; blocks of 256 threads 152 / 146 / 39; a
+// register limit that spills costs up to 2x.
 constexpr int kUnroll[2] = {4, 2};
-constexpr int kBlocks[2] = {2, 3};
+constexpr int kBlocks[2] = {4, 6};
 constexpr int kWant[2] = {160, 64};
 
 template <class T>
