@@ -268,6 +268,11 @@ __device__ __forceinline__ float4 cluster_load4(uint32_t at, int rank) {
     return x;
 }
 
+// Weights are held 2^kLift above the row's reference: fp16 ends at 2^-24, which many small weights of a long row
+// would reach together (the reference is within 2^8 of the largest, so 2^15 stays below fp16's 2^16).
+template <class T>
+constexpr float kLift = std::is_same<T, half>::value ? 7.f : 0.f;
+
 // 16-bit pairs of the two element types.
 template <class T>
 struct Pair;

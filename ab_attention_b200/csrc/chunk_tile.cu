@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             const int32_t whole_end = job.low[g].end, whole_low = job.high[g].low, whole_sink = job.low[g].sink;
             const int32_t head = job.t.head, after = job.t.base - head * kKeys, begin = job.begin;
             float m = -INFINITY;   // the row's reference, a bare score
-            float mk = 0.f;        // m * kappa, 0 while m is -inf
+            float mk = 0.f;        // m * kappa - kLift, 0 while m is -inf
             float l = 0.f;
 #pragma unroll 1
             for (int i = 0; i < n; ++i) {
@@ -682,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     const float next = grow ? top : m;
                     const float scale = grow ? exp2f((m - next) * a.kappa) : 1.0f;
                     m = next;
-                    mk = m == -INFINITY ? 0.f : m * a.kappa;
+                    mk = m == -INFINITY ? 0.f : m * a.kappa - kLift<T>;
                     l *= scale;
                     if (i > 0 && __any_sync(0xffffffffu, grow)) {
                         if (!wait(kBarO + g, tiles + i - 1)) {
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     // o = O / l, unless the scores are so large that it reaches whole units.
                     shift = mk;
                     if (!(fabsf(mk) < kLargeScore)) {
-                        shift = 0.f;
+                        shift = -kLift<T>;
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
                             r0[e] = __float_as_uint(__uint_as_float(r0[e]) - m);

@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
                     const float shift = m[x][h] == -INFINITY ? 0.f : m[x][h];
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        const float p0 = exp2f((s[x][y][2 * h] - shift) * a.kappa);
-                        const float p1 = exp2f((s[x][y][2 * h + 1] - shift) * a.kappa);
+                        const float p0 = exp2f(fmaf(s[x][y][2 * h] - shift, a.kappa, kLift<T>));
+                        const float p1 = exp2f(fmaf(s[x][y][2 * h + 1] - shift, a.kappa, kLift<T>));
                         l[x][h] += p0 + p1;
                         p[x][2 * y + h] = Pair<T>::pack(p0, p1);
                         const float2 r = Pair<T>::unpack(p[x][2 * y + h]);
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
                 l[x][h] += __shfl_xor_sync(0xffffffffu, l[x][h], 2);
                 if ((lane & 3) == 0) {
                     const int r = 16 * x + 8 * h + (lane >> 2);
-                    stat_m[warp * L::rows + r] = m[x][h] * a.kappa;
+                    stat_m[warp * L::rows + r] = m[x][h] * a.kappa - kLift<T>;
                     stat_l[warp * L::rows + r] = l[x][h];
                 }
             }

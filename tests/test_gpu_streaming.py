@@ -254,6 +254,23 @@ def test_many_ragged_chunks(heads, kv, page):
         assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
 
 
+@pytest.mark.parametrize("tokens", [1, 300])
+@pytest.mark.parametrize("dtype", [BF, HALF])
+def test_many_small_weights(tokens, dtype):
+    """One key outweighs each of 60,000 others 2^22.6 times, and they make up the result. fp16 ends at 2^-24:
+    weights are lifted by 2^7, so each is off by at most 2^-25 / 2^7 of the largest (bf16 keeps its 2^-8 of each)."""
+    keys = 60000
+    q, k = torch.ones(1, 1, tokens, 128, dtype=dtype, device="cuda"), torch.zeros(1, 1, keys, 128, dtype=dtype, device="cuda")
+    v = torch.ones_like(k)
+    k[:, :, 0], v[:, :, 0] = 1.384765625, 0
+    o, lse = ab.window_attention(q, k, v, return_lse=True)
+    ref, ref_lse, a = stream.attend(q[0].transpose(0, 1), k[0].transpose(0, 1), v[0].transpose(0, 1))
+    u = half_step(dtype)
+    tol = (2.02 * u + 4e-4) * a + (keys * 2 ** -32 if dtype == HALF else 0)
+    assert ((o[0].transpose(0, 1).double() - ref).abs() <= tol).all()
+    assert ((lse[0].T.double() - ref_lse).abs() <= 5e-4).all()
+
+
 def test_window_attention_of_nothing():
     empty = torch.empty(2, 4, 0, 128, dtype=BF, device="cuda")
     q = torch.randn(2, 4, 3, 128, device="cuda").to(BF)
