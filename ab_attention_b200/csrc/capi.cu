@@ -801,14 +801,31 @@ int abx_rotary(const abx_rotary_args* r, abx_stream_t stream) {
             dims += r->sections[x];
         }
         if (dims != abx::kHeadDim) return fail(ABX_ERR_INVALID_ARGUMENT, "sections must sum to 128 (got %d)", dims);
-        const double log_theta = std::log(r->theta);
-        int pair = 0;
-        for (int x = 0; x < r->axes; ++x)
-            for (int i = 0; i < r->sections[x] / 2; ++i, ++pair) {
-                const double power = r->shared ? 2.0 * pair / abx::kHeadDim : 2.0 * i / r->sections[x];
-                a.freq[pair] = std::exp(-power * log_theta) / 3.14159265358979323846;
-                a.axis[pair] = static_cast<uint8_t>(x);
-            }
+        // The frequencies follow from the axes alone: worked out when those change (0.7 us of a call's host time).
+        struct Table {
+            int32_t axes, sections[abx::kRotaryAxes], shared;
+            double theta;
+            double freq[abx::kPairs];
+            uint8_t axis[abx::kPairs];
+        };
+        thread_local Table table{};
+        if (table.axes != r->axes || table.shared != (r->shared != 0) || table.theta != r->theta ||
+            std::memcmp(table.sections, r->sections, sizeof(int32_t) * r->axes) != 0) {
+            const double log_theta = std::log(r->theta);
+            int pair = 0;
+            for (int x = 0; x < r->axes; ++x)
+                for (int i = 0; i < r->sections[x] / 2; ++i, ++pair) {
+                    const double power = r->shared ? 2.0 * pair / abx::kHeadDim : 2.0 * i / r->sections[x];
+                    table.freq[pair] = std::exp(-power * log_theta) / 3.14159265358979323846;
+                    table.axis[pair] = static_cast<uint8_t>(x);
+                }
+            table.axes = r->axes;
+            table.shared = r->shared != 0;
+            table.theta = r->theta;
+            std::memcpy(table.sections, r->sections, sizeof(int32_t) * r->axes);
+        }
+        std::memcpy(a.freq, table.freq, sizeof(a.freq));
+        std::memcpy(a.axis, table.axis, sizeof(a.axis));
     }
     auto add = [&](const char* name, const void* src, const int64_t (&s)[3], void* dst, const int64_t (&d)[3],
                    int64_t heads, bool turn, bool to_cache) -> int {

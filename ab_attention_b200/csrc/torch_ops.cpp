@@ -11,6 +11,7 @@
 // Only CUDA kernels are registered: a CPU tensor finds no kernel and raises, so
 // there is no silent fallback. Meta kernels give the output shapes to tracers.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -157,6 +158,11 @@ std::tuple<at::Tensor, at::Tensor> sparse_prefill_cuda(const at::Tensor& q, cons
 // ---- streaming operators: rotary positions, cache append, chunk and window attention -------
 // Argument errors raise ValueError. The checks are shared with the Meta kernels.
 
+// A new CUDA tensor on `like`'s device, without another trip through the dispatcher (half a microsecond a tensor).
+at::Tensor fresh(at::IntArrayRef size, at::ScalarType dtype, const at::Tensor& like) {
+    return at::Tensor(at::detail::empty_cuda(size, dtype, like.device(), std::nullopt));
+}
+
 int dtype_code(const at::Tensor& t, const char* name, bool f32 = false) {
     if (t.scalar_type() == at::kBFloat16) return ABX_BF16;
     if (t.scalar_type() == at::kHalf) return ABX_FP16;
@@ -244,8 +250,8 @@ std::tuple<at::Tensor, at::Tensor> rotary_cuda(const at::Tensor& q, const std::o
                                                bool shared, bool halves, bool inverse) {
     check_rotary(q, k, positions, sections, theta);
     c10::cuda::CUDAGuard guard(q.device());
-    auto q_out = at::empty(q.sizes(), q.options());
-    auto k_out = k ? at::empty(k->sizes(), k->options()) : at::empty({0}, q.options());
+    auto q_out = fresh(q.sizes(), q.scalar_type(), q);
+    auto k_out = fresh(k ? k->sizes() : at::IntArrayRef({0}), q.scalar_type(), q);
     abx_rotary_args r{};
     r.dtype = dtype_code(q, "q", true);
     set_axes(r, sections, theta, shared, halves, inverse);
@@ -330,7 +336,7 @@ at::Tensor append_cuda(at::Tensor keys, at::Tensor values, const at::Tensor& k, 
                        at::IntArrayRef sections, double theta, bool shared, bool halves) {
     check_append(keys, values, k, v, page_table, starts, lengths, q, positions, sections, theta);
     c10::cuda::CUDAGuard guard(keys.device());
-    auto q_out = q ? at::empty(q->sizes(), q->options()) : at::empty({0}, keys.options());
+    auto q_out = fresh(q ? q->sizes() : at::IntArrayRef({0}), keys.scalar_type(), keys);
     if (k.size(0) == 0 || page_table.size(0) == 0) {
         TORCH_CHECK_VALUE(k.size(0) == 0, "tokens without a sequence");
         return q_out;
@@ -384,7 +390,7 @@ void attend(abx_chunk_args& c, const at::Tensor& q) {
     size_t bytes = 0;
     check_status(abx_chunk_workspace_size(&c, &bytes), "abx_chunk_workspace_size");
     at::Tensor ws;
-    if (bytes > 0) ws = workspace(static_cast<int64_t>(bytes), q);
+    if (bytes > 0) ws = fresh({static_cast<int64_t>(bytes) + 256}, at::kByte, q);
     check_status(abx_chunk_attention(&c, bytes > 0 ? aligned256(ws) : nullptr, bytes, stream_of(q)), "abx_chunk_attention");
 }
 
@@ -449,8 +455,9 @@ void chunk_attention_out_cuda(const at::Tensor& q, const at::Tensor& keys, const
 
 std::tuple<at::Tensor, at::Tensor> chunk_results(const at::Tensor& q, bool lse) {
     TORCH_CHECK_VALUE(q.dim() == 3, "q must be [tokens, heads, 128] (got ", q.sizes(), ")");
-    return {at::empty(q.sizes(), q.options()),
-            lse ? at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat)) : at::Tensor()};
+    if (q.is_meta())
+        return {at::empty(q.sizes(), q.options()), at::empty({lse ? q.size(0) : 0, q.size(1)}, q.options().dtype(at::kFloat))};
+    return {fresh(q.sizes(), q.scalar_type(), q), fresh({lse ? q.size(0) : 0, q.size(1)}, at::kFloat, q)};
 }
 
 std::tuple<at::Tensor, at::Tensor> chunk_attention_cuda(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values,
@@ -460,7 +467,7 @@ std::tuple<at::Tensor, at::Tensor> chunk_attention_cuda(const at::Tensor& q, con
     auto [out, lse] = chunk_results(q, want_lse);
     chunk_attention_out_cuda(q, keys, values, page_table, starts, lengths, longest, window, sinks, block, out,
                              want_lse ? std::optional<at::Tensor>(lse) : std::nullopt);
-    return {out, want_lse ? lse : at::empty({0}, q.options().dtype(at::kFloat))};
+    return {out, lse};
 }
 
 void check_window(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t sinks, int64_t block) {
@@ -479,8 +486,8 @@ std::tuple<at::Tensor, at::Tensor> window_attention_cuda(const at::Tensor& q, co
                                                          int64_t window, int64_t sinks, int64_t block) {
     check_window(q, k, v, window, sinks, block);
     c10::cuda::CUDAGuard guard(q.device());
-    auto out = at::empty(q.sizes(), q.options());
-    auto lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+    auto out = fresh(q.sizes(), q.scalar_type(), q);
+    auto lse = fresh({q.size(0), q.size(1), q.size(2)}, at::kFloat, q);
     if (q.numel() == 0) return {out, lse};
     if (k.numel() == 0) return {out.zero_(), lse.fill_(-std::numeric_limits<float>::infinity())};
     const auto qr = as_rows(q, false), kr = as_rows(k, true), vr = as_rows(v, true);
@@ -539,7 +546,7 @@ std::tuple<at::Tensor, at::Tensor> chunk_attention_meta(const at::Tensor& q, con
     auto [out, lse] = chunk_results(q, want_lse);
     check_chunk(q, keys, values, page_table, starts, lengths, longest, window, sinks, block, out,
                 want_lse ? std::optional<at::Tensor>(lse) : std::nullopt);
-    return {out, want_lse ? lse : at::empty({0}, q.options().dtype(at::kFloat))};
+    return {out, lse};
 }
 
 std::tuple<at::Tensor, at::Tensor> window_attention_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
