@@ -886,8 +886,7 @@ int abx_chunk_attention(const abx_chunk_args* args, void* workspace, size_t work
     }
     a.error = abx::device_error_word();
     const bool fp16 = args->dtype == ABX_FP16;
-    const int tile_keys = abx::chunk_tile_keys(a);
-    const int box_rows = a.table == nullptr || a.page_size > tile_keys ? tile_keys : a.page_size;
+    const int box_rows = a.table == nullptr || a.page_size > abx::kChunkBoxKeys ? abx::kChunkBoxKeys : a.page_size;
     const int64_t tokens = a.table == nullptr ? a.keys : a.page_size;
     abx::ChunkMaps maps{};
     if (int st = check_cuda(encode_cache(&maps.k, args->k, fp16, tokens, a.kv_heads, a.pages, args->k_stride, box_rows),

@@ -54,6 +54,7 @@ constexpr int32_t kMaxCacheKeys = 0x3fffffff;
 constexpr int kMaxCluster = 8;
 constexpr int kChunkTokenKeys = 64;  // keys of a tile of each kernel
 constexpr int kChunkTileKeys = 128;
+constexpr int kChunkBoxKeys = 64;    // keys of a TMA box at most: a tile of the one kernel, half a tile of the other
 
 // One tile of rows of one sequence.
 struct ChunkUnit {

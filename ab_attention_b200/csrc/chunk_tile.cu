@@ -25,9 +25,12 @@
 // between two tiles of rows otherwise cost 15,000 cycles (five tiles of keys): now the
 // next queries (TMA), keys and first scores arrive during the last tile, and four
 // warps of their own write finished rows during the next one. 8,191 tokens in a
-// window of 1,024 (ten tiles of keys each): 140 us with one CTA a tile of rows, 105 us so.
-// The code is kept small (100 KB; 159 KB cost 3 to 10%): a change of jobs runs code that
+// window of 1,024 (ten tiles of keys each): 140 us with one CTA a tile of rows, 104 us so.
+// The code is kept small (90 KB; 159 KB cost 3 to 10%): a change of jobs runs code that
 // is not in the instruction cache.
+//
+// Keys are walked in halves of a tile (a box of 64), whatever lies between two: a window's sinks share a
+// tile with its last keys, which makes nine tiles of those ten (96 us).
 //
 // The maximum of a row is raised lazily (only when it grows by more than 2^8, so P stays
 // in fp16's range and O is rarely rescaled); sums and O are f32. P is rounded to the
@@ -43,6 +46,7 @@ namespace {
 constexpr int kGroups = 2;
 constexpr int kGroupRows = 128;
 constexpr int kKeys = kChunkTileKeys;
+constexpr int kHalf = kChunkBoxKeys;  // the keys of a tile's halves need not adjoin: a window's sinks and its last keys share one
 constexpr int kMmaWarp = 8;    // one warp a group
 constexpr int kLoadWarp = 10;  // one for K, one for V
 constexpr int kOutWarp = 12;   // four warps: finished rows; the first also finds the next job and loads its queries
@@ -88,7 +92,7 @@ struct Job {
     KeyTiles t;
     Seen low[kGroups], high[kGroups];  // of the first and last row of each group
     int32_t kvh, split, rows, whole;
-    int32_t begin, n;                  // key tiles; n < 0: no more jobs
+    int32_t begin, n;                  // key tiles of two halves each (t counts halves); n < 0: no more jobs
 };
 constexpr uint32_t kOffTmem = kOffJobs + 2 * sizeof(Job);
 constexpr uint32_t kOffAbort = kOffTmem + 4;
@@ -96,6 +100,7 @@ constexpr uint32_t kOffSums = (kOffAbort + 4 + 15) / 16 * 16;  // [group][row]: 
 constexpr uint32_t kSmemBytes = kOffSums + kGroups * kGroupRows * 8;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory exceeds the per-block limit");
 constexpr uint32_t kTmemColumns = 512;
+static_assert(kKeys == 2 * kHalf, "a tile is two boxes of keys");
 __device__ __forceinline__ constexpr uint32_t col_o(int g) { return 128u * static_cast<uint32_t>(g); }
 __device__ __forceinline__ constexpr uint32_t col_s(int g) { return 256u + 128u * static_cast<uint32_t>(g); }
 constexpr uint64_t kWaitLimit = 400ull * 1000 * 1000;  // cycles, of the waits at a CTA's end
@@ -261,11 +266,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 const int begin = job.begin, kvh = job.kvh;
                 done_with(j);
                 int32_t page = 0, row = 0;
+                const int half = lane * box_rows >= kHalf, in_half = lane * box_rows - half * kHalf;
                 auto look_up = [&](int i) {
-                    const int32_t k0 = t.key<kKeys>(begin + i);
-                    page = lane < boxes ? chunk_page(a, u, t, k0 + lane * box_rows, box_rows) : 0;
-                    // a page of 128 keys and less is a box of its own and starts at its first row
-                    row = boxes > 1 ? 0 : chunk_page_row(a, k0);
+                    if (lane >= boxes) return;
+                    const int32_t k = t.key<kHalf>(2 * (begin + i) + half) + in_half;
+                    page = chunk_page(a, u, t, k, box_rows);
+                    row = chunk_page_row(a, k);
                 };
                 if (n > 0) look_up(0);
 #pragma unroll 1
@@ -280,9 +286,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     __syncwarp();
 #pragma unroll 1
                     for (int b = 0; b < boxes; ++b) {
-                        const int32_t p = __shfl_sync(0xffffffffu, page, b);
-                        tma_load_4d_elect(to + b * box_rows * 128, map, 0, row, kvh, p, full);
-                        tma_load_4d_elect(to + kSlab + b * box_rows * 128, map, 64, row, kvh, p, full);
+                        const int32_t p = __shfl_sync(0xffffffffu, page, b), y = __shfl_sync(0xffffffffu, row, b);
+                        tma_load_4d_elect(to + b * box_rows * 128, map, 0, y, kvh, p, full);
+                        tma_load_4d_elect(to + kSlab + b * box_rows * 128, map, 64, y, kvh, p, full);
                     }
                     if (i + 1 < n) look_up(i + 1);  // while that tile's place is still taken
                 }
@@ -322,9 +328,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     return Seen{__shfl_sync(0xffffffffu, bound.sink, from), __shfl_sync(0xffffffffu, bound.low, from),
                                 __shfl_sync(0xffffffffu, bound.end, from)};
                 };
-                t = chunk_tiles<kKeys>(a, of(0), of(1));
+                t = chunk_tiles<kHalf>(a, of(0), of(1));
                 int end;
-                whole = chunk_part(a, t.count, z, begin, end);
+                whole = chunk_part(a, (t.count + 1) / 2, z, begin, end);
                 n = end - begin;
                 if (whole && z > 0) rows = n = 0;  // nothing to do
             };
@@ -620,15 +626,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 continue;
             }
             const Seen mine = chunk_seen(a, job.u, g_row0 + min(r, g_rows - 1));
-            // Tiles in [whole_low, whole_end) or below whole_sink are seen whole by all rows of the group.
+            // Halves in [whole_low, whole_end) or below whole_sink are seen whole by all rows of the group.
             const int32_t whole_end = job.low[g].end, whole_low = job.high[g].low, whole_sink = job.low[g].sink;
-            const int32_t head = job.t.head, after = job.t.base - head * kKeys, begin = job.begin;
+            const int32_t head = job.t.head, after = job.t.base - head * kHalf, begin = job.begin;
             float m = -INFINITY;   // the row's reference, a bare score
             float mk = 0.f;        // m * kappa - kLift, 0 while m is -inf
             float l = 0.f;
 #pragma unroll 1
             for (int i = 0; i < n; ++i) {
-                const int32_t k0 = (begin + i) * kKeys + (begin + i < head ? 0 : after);
+                const int h = 2 * (begin + i);
+                const int32_t k0 = h * kHalf + (h < head ? 0 : after), k1 = (h + 1) * kHalf + (h + 1 < head ? 0 : after);
                 if (!wait(kBarS + g, tiles + i)) {
                     ok = false;
                     break;
@@ -647,7 +654,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 tc::fence_before_sync();
                 tc::mbar_arrive(bar(kBarSFree + g));
                 // Keys that the row does not see -> -inf (only in tiles that some row does not see whole).
-                const bool partly = k0 + kKeys > whole_end || (k0 < whole_low && k0 + kKeys > whole_sink);
+                const bool partly = max(k0, k1) + kHalf > whole_end || (k0 < whole_low && k0 + kHalf > whole_sink) ||
+                                    (k1 < whole_low && k1 + kHalf > whole_sink);
                 if (partly) {
                     auto hide = [&](uint32_t (&x)[32], int first) {
                         const uint32_t see = low_bits(mine.end - first) & (~low_bits(mine.low - first) | low_bits(mine.sink - first));
@@ -658,8 +666,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     };
                     hide(r0, k0);
                     hide(r1, k0 + 32);
-                    hide(r2, k0 + 64);
-                    hide(r3, k0 + 96);
+                    hide(r2, k1);
+                    hide(r3, k1 + 32);
                 }
                 float top;
                 {
@@ -765,13 +773,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 // V rows that no row sees (a page's stale tail) must not meet P = 0 as NaN or infinity. Both
                 // groups clear them, each before its own product.
                 const KeyTiles& t = job.t;
-                if (partly && (!t.any(k0) || !t.any(k0 + kKeys - 1) || (k0 < t.first.low && k0 + kKeys > t.last.sink))) {
+                auto gaps = [&](int32_t k) {  // of a half
+                    return !t.any(k) || !t.any(k + kHalf - 1) || (k < t.first.low && k + kHalf > t.last.sink);
+                };
+                if (partly && (gaps(k0) || gaps(k1))) {
                     const int st = (keys + i) % kVStages;
                     if (!wait(kBarV + st, (keys + i) / kVStages)) {
                         ok = false;
                         break;
                     }
-                    if (!t.any(k0 + r)) {
+                    if (!t.any((r < kHalf ? k0 : k1 - kHalf) + r)) {
                         const uint32_t v_row = base + kOffV + st * kOperand + r * 128;
 #pragma unroll
                         for (int c = 0; c < 16; ++c)  // in an order without bank conflicts

@@ -378,6 +378,27 @@ def test_pages_behind_the_window_may_be_gone(new, heads):
     b.check(want, None, **rule)
 
 
+@pytest.mark.parametrize("page", [16, 64, 128, 256, None])
+@pytest.mark.parametrize("sinks,window", [(1, 1000), (64, 190), (65, 64), (130, 333), (190, 1)])
+@pytest.mark.parametrize("new", [7, 290])
+def test_sinks_beside_a_window(new, sinks, window, page):
+    """The sinks' keys and the window's lie in one tile, and what lies between, which no token sees, is NaN."""
+    n, heads, kv = 1733, 8, 2
+    b = Batch(new + sinks, [(new, n)], heads, kv, page or 16, BF)
+    rule = {"window": window, "sinks": sinks, "block": 1}
+    hidden = range(sinks, n - new + 1 - window)
+    if page:
+        for j in hidden:
+            at = b.table[0, j // page].item()
+            b.keys[at, :, j % page] = b.values[at, :, j % page] = math.nan
+        b.check(*ab.chunk_attention(b.q, b.cache, *b.plan, longest=new, return_lse=True, **rule), **rule)
+        return
+    q, k, v = (x.transpose(0, 1)[None].contiguous() for x in (b.q, b.k[0], b.v[0]))
+    k[:, :, hidden.start:hidden.stop] = v[:, :, hidden.start:hidden.stop] = math.nan
+    o, lse = ab.window_attention(q, k, v, return_lse=True, **rule)
+    b.check(o[0].transpose(0, 1), lse[0].T, **rule)
+
+
 @pytest.mark.parametrize("new", [1, 50])
 def test_bad_pages_lengths_and_chunks_are_reported(new):
     """What the device finds wrong is reported in the device error word, and nothing is read or
