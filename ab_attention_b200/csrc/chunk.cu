@@ -1,4 +1,6 @@
 // Which kernel takes a chunk call, how its keys are shared out to CTAs, and how the shares are joined.
+#include <algorithm>
+
 #include "chunk.cuh"
 
 namespace abx {
@@ -18,6 +20,57 @@ constexpr int kRaggedTiles = 16;
 // Jobs an SM for ragged chunks on the tile kernel, if all were as long as the table allows: nine of 30 to 701 tokens
 // over up to 8,000 keys take 188 / 188 / 195 / 195 us with 2 / 3 / 4 / 5, and 211 us unsplit.
 constexpr int kRaggedJobs = 3;
+// Waves of row tiles up to which a last wave that leaves half the SMs idle may be taken in halves: half a row tile
+// takes 0.77 of a whole one's time, so that saves a quarter of a wave at most. 12 heads, 3,600 tokens on themselves (1.2
+// waves): 115 us whole, 102.5 us; 24 heads, 1,700 causal (1.1): 48.4 / 41; 16 heads on 4, 8,191 in a window of 1,024
+// (3.5): 87.6 / 84.1.
+constexpr int kHalvesUpTo = 5;
+
+// Whether the call's row tiles, each taken by the SM that is free first, end sooner when those from job `whole` on
+// are taken as two halves. Not always: short row tiles (the first tokens under a causal mask) may fill the last wave
+// already, and halves cost half as much again (4 heads, 20,000 tokens in a window of 2,000: 97.7 us whole, 105 us).
+bool halves_end_sooner(const ChunkArgs& a, int jobs, int whole) {
+    constexpr int kLongest = 64, kRing = 128;  // ticks of the longest row tile
+    const int units = jobs / a.kv_heads, half = a.tile_rows / 2, rows = std::min(a.longest * a.group, units * a.tile_rows);
+    const int per = (rows + a.tile_rows - 1) / a.tile_rows;  // row tiles of a sequence, the last first
+    // In 1/13 of a whole tile's step on 128 keys: about three steps to start and end, and ten for half the rows.
+    auto cost = [&](int row0, int count) -> int {
+        const int past = std::min(row0 + count, rows);
+        if (past <= row0) return 0;
+        auto end = [&](int row) {
+            const int p = a.keys - a.longest + row / a.group;
+            return p < 0 ? 0 : std::min(a.block == 1 ? p + 1 : (p / a.block + 1) * a.block, a.keys);
+        };
+        const int low = std::max(end(row0) - a.window, 0), keys = end(past - 1) - low + std::min(a.sinks, low);
+        return 39 + (keys + kChunkTileKeys - 1) / kChunkTileKeys * (past - row0 <= half ? 10 : 13);
+    };
+    int of[kHalvesUpTo * kSms], longest = 1;
+    for (int x = 0; x < per; ++x) longest = std::max(longest, of[x] = cost((per - 1 - x) * a.tile_rows, a.tile_rows));
+    const float scale = static_cast<float>(kLongest - 1) / longest;
+    auto ticks = [&](int c) { return c == 0 ? 0 : static_cast<int>(c * scale) + 1; };
+    for (int x = 0; x < per; ++x) of[x] = ticks(of[x]);
+    struct Sms {
+        int16_t free[kRing] = {kSms};  // that become free at a tick
+        int now = 0, end = 0;
+        void run(int t) {
+            if (t == 0) return;
+            while (free[now % kRing] == 0) ++now;
+            --free[now % kRing];
+            ++free[(now + t) % kRing];
+            end = std::max(end, now + t);
+        }
+    } with, without;
+    int x = 0;  // the row tile of its sequence
+    for (int j = 0; j < whole; ++j, x = x + 1 == per ? 0 : x + 1) without.run(of[x]);
+    with = without;
+    for (int j = whole; j < jobs; ++j, x = x + 1 == per ? 0 : x + 1) {
+        const int row0 = (per - 1 - x) * a.tile_rows;
+        without.run(of[x]);
+        with.run(ticks(cost(row0, half)));
+        with.run(ticks(cost(row0 + half, half)));
+    }
+    return with.end < without.end;
+}
 
 // Joins the splits of each row: o = sum_s 2^(lse_s - lse) o_s. A block a row, four dims a lane, each warp an
 // eighth of the splits; reads splits * 516 bytes a row.
@@ -258,8 +311,16 @@ void chunk_layout(ChunkArgs& a) {
 int chunk_tile_keys(const ChunkArgs& a) { return a.tile_rows < 256 ? kChunkTokenKeys : kChunkTileKeys; }
 
 cudaError_t launch_chunk(const ChunkArgs& a, const ChunkMaps& maps, bool fp16, int box_rows, cudaStream_t stream) {
-    return a.tile_rows < 256 ? launch_chunk_token(a, maps, fp16, box_rows, stream)
-                             : launch_chunk_tile(a, maps, fp16, box_rows, stream);
+    if (a.tile_rows < 256) return launch_chunk_token(a, maps, fp16, box_rows, stream);
+    ChunkArgs b = a;
+    const int64_t ctas = chunk_units(a) * a.kv_heads, over = ctas % kSms;
+    const bool ragged = a.starts != nullptr && a.seqs > 1;
+    if (a.splits == 1 && !ragged && over > 0 && 2 * over <= kSms && ctas <= kHalvesUpTo * kSms &&
+        halves_end_sooner(a, static_cast<int>(ctas), static_cast<int>(ctas - over))) {
+        b.units = static_cast<int32_t>(ctas / a.kv_heads);
+        b.whole_jobs = static_cast<int32_t>(ctas - over);
+    }
+    return launch_chunk_tile(b, maps, fp16, box_rows, stream);
 }
 
 cudaError_t launch_chunk_join(const ChunkArgs& a, bool fp16, cudaStream_t stream) {

@@ -43,6 +43,8 @@ struct ChunkArgs {
     int32_t splits;        // CTAs that share the keys of one row tile
     int32_t cluster;       // 1: the splits of a row tile form a cluster and join their rows themselves
     int32_t span;          // key tiles of one split, or 0: the row tile's keys in equal parts
+    int32_t units;         // > 0: a grid of one dimension, `units` row tiles a key head, and from the
+    int32_t whole_jobs;    // whole_jobs-th on each row tile as two of half its rows (the tile kernel)
     int32_t q_map;         // 1: maps.q describes the queries (the tile kernel, group divides 128)
     int64_t rows_total;    // tokens of all sequences * heads
     float kappa;           // 128^-0.5 * log2(e)

@@ -315,8 +315,20 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             int rows = 0, begin = 0, n = 0;
             bool whole = false;
             auto work_out = [&]() {
+                int most = kGroups * kGroupRows, second = 0;
+                if (a.units > 0) {
+                    const int past = x - a.whole_jobs;
+                    if (past >= 0) {
+                        most = kGroupRows;
+                        second = past & 1;
+                        x = a.whole_jobs + (past >> 1);
+                    }
+                    y = x / a.units;
+                    x -= y * a.units;
+                }
                 u = chunk_unit(a, x, kGroups * kGroupRows);
-                rows = u.seq < 0 ? 0 : min(kGroups * kGroupRows, u.n * a.group - u.row0);
+                u.row0 += second * kGroupRows;
+                rows = u.seq < 0 ? 0 : min(most, u.n * a.group - u.row0);
                 n = begin = 0;
                 whole = false;
                 if (rows <= 0) return;
@@ -825,7 +837,9 @@ cudaError_t launch(const ChunkArgs& a, const ChunkMaps& maps, int box_rows, cuda
     if (attr.numRegs * kThreads < 8 * 32 * kSoftmaxRegs + (kThreads - 8 * 32) * kOtherRegs) return cudaErrorInvalidConfiguration;
     const int64_t units = chunk_units(a);
     if (units > 0x7fffffff || a.splits > 65535) return cudaErrorInvalidConfiguration;
-    kernel<<<dim3(static_cast<unsigned>(units), a.kv_heads, a.splits), kThreads, kSmemBytes, stream>>>(a, maps, box_rows);
+    const dim3 grid = a.units > 0 ? dim3(static_cast<unsigned>(2 * units * a.kv_heads - a.whole_jobs))
+                                  : dim3(static_cast<unsigned>(units), a.kv_heads, a.splits);
+    kernel<<<grid, kThreads, kSmemBytes, stream>>>(a, maps, box_rows);
     return cudaGetLastError();
 }
 

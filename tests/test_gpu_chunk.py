@@ -226,6 +226,24 @@ def test_nan_in_a_query_stays_in_its_row(tokens, keys):
     assert torch.equal(o, want) and torch.equal(lse, want_lse)
 
 
+@pytest.mark.parametrize("batch,heads,kv,tokens,keys,rule", [
+    (1, 12, 12, 1000, 1000, {"block": 1000}),           # fewer row tiles than half the SMs
+    (2, 12, 4, 1045, 1300, {"window": 700, "sinks": 5}),  # 3 heads a key head: queries loaded one by one
+    (1, 16, 4, 1032, 1032, {}),                         # 16.1 row tiles a key head: the last half has no rows
+    (1, 38, 38, 1025, 1025, {"window": 400}),           # 190 row tiles, 42 of them in the last wave
+    (3, 20, 20, 700, 700, {"block": 70}),               # 180 row tiles of three sequences
+])
+def test_row_tiles_in_halves(batch, heads, kv, tokens, keys, rule):
+    """The row tiles of a last wave are taken in halves."""
+    g = gen(tokens + heads)
+    q = normal(g, batch, heads, tokens, 128)
+    k, v = (normal(g, batch, kv, keys, 128) for _ in range(2))
+    rule = {"window": None, "sinks": 0, "block": 1} | rule
+    o, lse = ab.window_attention(q, k, v, return_lse=True, **rule)
+    for b in range(batch):
+        hold(o[b].transpose(0, 1), lse[b].T, *(x[b].transpose(0, 1) for x in (q, k, v)), **rule)
+
+
 @pytest.mark.parametrize("heads,kv,tokens,keys,window,sinks,block", [
     (36, 36, 1500, 1500, 100, 3, 1), (40, 8, 1100, 1400, None, 0, 1), (24, 2, 777, 777, 33, 130, 64), (70, 14, 900, 300, None, 0, 1),
 ])
