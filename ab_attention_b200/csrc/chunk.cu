@@ -17,9 +17,6 @@ constexpr int kRaggedWaves = 8;
 // ... unless no part of the longest has more tiles than this without them: a part of 16 tiles takes 12 us, a join
 // with its launch 8 us more.
 constexpr int kRaggedTiles = 16;
-// Jobs an SM for ragged chunks on the tile kernel, if all were as long as the table allows: nine of 30 to 701 tokens
-// over up to 8,000 keys take 188 / 188 / 195 / 195 us with 2 / 3 / 4 / 5, and 211 us unsplit.
-constexpr int kRaggedJobs = 3;
 // Waves of row tiles up to which a last wave that leaves half the SMs idle may be taken in halves: half a row tile
 // takes 0.77 of a whole one's time, so that saves a quarter of a wave at most. 12 heads, 3,600 tokens on themselves (1.2
 // waves): 115 us whole, 102.5 us; 24 heads, 1,700 causal (1.1): 48.4 / 41; 16 heads on 4, 8,191 in a window of 1,024
@@ -285,26 +282,27 @@ void chunk_layout(ChunkArgs& a) {
         return;
     }
     // Equal parts, as many as make the waves of CTAs (one an SM) shortest: a part costs its tiles and
-    // about three more to start and end, joining costs a write and a read of each part's rows.
+    // about three more to start and end, joining costs a write and a read of each part's rows. Ragged: equal spans. The
+    // longest sequences come first, so the end is the longest job's, or the mean SM's and some of a job; the lengths,
+    // known on the device only, are taken as half the table's on average. Nine of 30 to 701 tokens over up to 8,000
+    // keys, 16 heads on 4: 159 us (one part) against 186 in the order of the sequences (two parts).
+    const bool ragged = a.starts != nullptr && a.seqs > 1;
+    a.sorted = ragged;
     a.span = 0;
     a.splits = 1;
-    if (a.starts != nullptr && a.seqs > 1) {
-        // Ragged: equal spans, so that the parts of long sequences come to about kRaggedJobs an SM and balance;
-        // a sequence within one span is not joined.
-        const int64_t want = ceil_div(static_cast<int64_t>(kSms) * kRaggedJobs, ctas), most = ceil_div(tiles, 8);
-        a.span = static_cast<int32_t>(ceil_div(tiles, want < most ? want : most));
-        a.splits = static_cast<int32_t>(ceil_div(tiles, a.span));
-        return;
-    }
     double best = 0;
-    for (int s = 1; s <= 16 && s <= tiles; ++s) {
-        const double waves = static_cast<double>(ceil_div(ctas * s, kSms));
+    for (int s = 1; s <= (ragged ? 32 : 16) && s <= tiles && (s == 1 || !ragged || 8 * (s - 1) < tiles); ++s) {
+        const double part = static_cast<double>(ceil_div(tiles, s)) + 3;
         const double join = s == 1 ? 0 : 2 + s * static_cast<double>(a.rows_total) * 1032 / 11e6;  // in tiles of 1.7 us
-        const double cost = waves * (static_cast<double>(ceil_div(tiles, s)) + 3) + join;
+        const double cost = join + (ragged ? std::max(part, ctas * (0.5 * tiles + 3) / kSms + part / 3) : ceil_div(ctas * s, kSms) * part);
         if (s == 1 || cost < 0.97 * best) {
             best = cost;
             a.splits = s;
         }
+    }
+    if (ragged) {
+        a.span = static_cast<int32_t>(ceil_div(tiles, a.splits));
+        a.splits = static_cast<int32_t>(ceil_div(tiles, a.span));
     }
 }
 
@@ -314,8 +312,7 @@ cudaError_t launch_chunk(const ChunkArgs& a, const ChunkMaps& maps, bool fp16, i
     if (a.tile_rows < 256) return launch_chunk_token(a, maps, fp16, box_rows, stream);
     ChunkArgs b = a;
     const int64_t ctas = chunk_units(a) * a.kv_heads, over = ctas % kSms;
-    const bool ragged = a.starts != nullptr && a.seqs > 1;
-    if (a.splits == 1 && !ragged && over > 0 && 2 * over <= kSms && ctas <= kHalvesUpTo * kSms &&
+    if (a.splits == 1 && !a.sorted && over > 0 && 2 * over <= kSms && ctas <= kHalvesUpTo * kSms &&
         halves_end_sooner(a, static_cast<int>(ctas), static_cast<int>(ctas - over))) {
         b.units = static_cast<int32_t>(ctas / a.kv_heads);
         b.whole_jobs = static_cast<int32_t>(ctas - over);

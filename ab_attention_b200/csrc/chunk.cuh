@@ -45,6 +45,8 @@ struct ChunkArgs {
     int32_t span;          // key tiles of one split, or 0: the row tile's keys in equal parts
     int32_t units;         // > 0: a grid of one dimension, `units` row tiles a key head, and from the
     int32_t whole_jobs;    // whole_jobs-th on each row tile as two of half its rows (the tile kernel)
+    int32_t sorted;        // 1: ragged sequences, the longest first; a grid of one dimension of splits, key heads and row
+                           // tiles, the first fastest (the tile kernel)
     int32_t q_map;         // 1: maps.q describes the queries (the tile kernel, group divides 128)
     int64_t rows_total;    // tokens of all sequences * heads
     float kappa;           // 128^-0.5 * log2(e)
@@ -80,8 +82,9 @@ __device__ __forceinline__ void chunk_sequence(const ChunkArgs& a, int s, int32_
 }
 
 // The row tile that unit u of the grid works on; called by whole warps. Tiles of
-// a sequence come last first: under a causal mask the longest rows start first.
-__device__ __forceinline__ ChunkUnit chunk_unit(const ChunkArgs& a, int u, int tile_rows) {
+// a sequence come last first: under a causal mask the longest rows start first. sorted: of every 32 sequences
+// those with the most keys come first.
+__device__ __forceinline__ ChunkUnit chunk_unit(const ChunkArgs& a, int u, int tile_rows, bool sorted) {
     ChunkUnit r{-1, 0, 0, 0, 0};
     if (a.starts == nullptr) {
         const int tiles = (a.tokens * a.group + tile_rows - 1) / tile_rows;
@@ -103,16 +106,26 @@ __device__ __forceinline__ ChunkUnit chunk_unit(const ChunkArgs& a, int u, int t
             if (bad) raise_device_error(a.error, ABX_ERR_INVALID_ARGUMENT);
             tiles = static_cast<int32_t>((static_cast<int64_t>(n) * a.group + tile_rows - 1) / tile_rows);
         }
-        int sum = tiles;
+        const int all = __reduce_add_sync(0xffffffffu, tiles);
+        if (before + all > u) {
+            int ahead = before;  // tiles of the sequences before this lane's
+            if (sorted) {
+#pragma unroll 1
+                for (int o = 0; o < 32; ++o) {
+                    const int other = __shfl_sync(0xffffffffu, len, o), its = __shfl_sync(0xffffffffu, tiles, o);
+                    if (other > len || (other == len && o < lane)) ahead += its;
+                }
+            } else {
+                int sum = tiles;
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const int other = __shfl_up_sync(0xffffffffu, sum, d);
-            if (lane >= d) sum += other;
-        }
-        const unsigned reached = __ballot_sync(0xffffffffu, before + sum > u);
-        if (reached) {
-            const int at = __ffs(reached) - 1;
-            const int tiles_before = before + __shfl_sync(0xffffffffu, sum - tiles, at);
+                for (int d = 1; d < 32; d *= 2) {
+                    const int other = __shfl_up_sync(0xffffffffu, sum, d);
+                    if (lane >= d) sum += other;
+                }
+                ahead += sum - tiles;
+            }
+            const int at = __ffs(__ballot_sync(0xffffffffu, u >= ahead && u - ahead < tiles)) - 1;
+            const int tiles_before = __shfl_sync(0xffffffffu, ahead, at);
             tiles = __shfl_sync(0xffffffffu, tiles, at);
             r.seq = base + at;
             r.row0 = (tiles - 1 - (u - tiles_before)) * tile_rows;
@@ -121,7 +134,7 @@ __device__ __forceinline__ ChunkUnit chunk_unit(const ChunkArgs& a, int u, int t
             r.first = __shfl_sync(0xffffffffu, first, at);
             return r;
         }
-        before += __shfl_sync(0xffffffffu, sum, 31);
+        before += all;
     }
     return r;
 }

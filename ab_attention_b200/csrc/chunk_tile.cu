@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
         } else if (warp >= kOutWarp) {
             // ---- the first of them: jobs. This CTA's own place in the grid, then the places of CTAs that have not
             // started. Tiles of rows fastest, then key heads, then splits: CTAs that run at the same time share K and V
-            // in L2, and the last parts of ragged sequences, short or empty, come last ----
+            // in L2. Ragged sequences go by length instead, so that no long job starts among the last ----
             int x = blockIdx.x, y = blockIdx.y, z = blockIdx.z;
             int asked[kGroups] = {0, 0};  // rounds of queries
             int questions = 0;
@@ -316,7 +316,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
             bool whole = false;
             auto work_out = [&]() {
                 int most = kGroups * kGroupRows, second = 0;
-                if (a.units > 0) {
+                if (a.sorted) {
+                    z = x % a.splits;
+                    x /= a.splits;
+                    y = x % a.kv_heads;
+                    x /= a.kv_heads;
+                } else if (a.units > 0) {
                     const int past = x - a.whole_jobs;
                     if (past >= 0) {
                         most = kGroupRows;
@@ -326,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                     y = x / a.units;
                     x -= y * a.units;
                 }
-                u = chunk_unit(a, x, kGroups * kGroupRows);
+                u = chunk_unit(a, x, kGroups * kGroupRows, a.sorted != 0);
                 u.row0 += second * kGroupRows;
                 rows = u.seq < 0 ? 0 : min(most, u.n * a.group - u.row0);
                 n = begin = 0;
@@ -837,8 +842,10 @@ cudaError_t launch(const ChunkArgs& a, const ChunkMaps& maps, int box_rows, cuda
     if (attr.numRegs * kThreads < 8 * 32 * kSoftmaxRegs + (kThreads - 8 * 32) * kOtherRegs) return cudaErrorInvalidConfiguration;
     const int64_t units = chunk_units(a);
     if (units > 0x7fffffff || a.splits > 65535) return cudaErrorInvalidConfiguration;
-    const dim3 grid = a.units > 0 ? dim3(static_cast<unsigned>(2 * units * a.kv_heads - a.whole_jobs))
-                                  : dim3(static_cast<unsigned>(units), a.kv_heads, a.splits);
+    if (a.sorted && units * a.kv_heads * a.splits > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    const dim3 grid = a.sorted      ? dim3(static_cast<unsigned>(units * a.kv_heads * a.splits))
+                      : a.units > 0 ? dim3(static_cast<unsigned>(2 * units * a.kv_heads - a.whole_jobs))
+                                    : dim3(static_cast<unsigned>(units), a.kv_heads, a.splits);
     kernel<<<grid, kThreads, kSmemBytes, stream>>>(a, maps, box_rows);
     return cudaGetLastError();
 }

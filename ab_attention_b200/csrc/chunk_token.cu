@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.z, kvh = blockIdx.y;
-    const ChunkUnit u = chunk_unit(a, blockIdx.x, L::rows);
+    const ChunkUnit u = chunk_unit(a, blockIdx.x, L::rows, false);
     if (u.seq < 0) return;  // past the last tile
     const int rows = min(L::rows, u.n * a.group - u.row0);
     const KeyTiles t = chunk_tiles<kKeys>(a, chunk_seen(a, u, u.row0), chunk_seen(a, u, u.row0 + rows - 1));

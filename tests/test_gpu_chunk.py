@@ -396,6 +396,20 @@ def test_pages_behind_the_window_may_be_gone(new, heads):
     b.check(want, None, **rule)
 
 
+@pytest.mark.parametrize("count,most,keys,heads,kv", [(2, 400, 900, 4, 4), (31, 90, 700, 8, 2), (40, 70, 300, 8, 4), (75, 45, 200, 12, 12)])
+def test_ragged_sequences_in_order_of_length(count, most, keys, heads, kv):
+    """Sequences of many lengths, some equal, some without tokens or keys: every 32 are taken longest first."""
+    sizes = []
+    for s in range(count):
+        new = s * 37 % (most + 1) if s % 5 else 0
+        sizes.append((new, 0 if s % 10 == 0 else max(new, s * 101 % (keys + 1) // 50 * 50)))
+    sizes[count // 2] = (most, keys)
+    b = Batch(count, sizes, heads, kv, 16, BF, behind=2)
+    for rule in ({"window": None, "sinks": 0, "block": 1}, {"window": 77, "sinks": 3, "block": 10}):
+        o, lse = ab.chunk_attention(b.q, b.cache, *b.plan, longest=most, return_lse=True, **rule)
+        b.check(o, lse, **rule)
+
+
 @pytest.mark.parametrize("page", [16, 64, 128, 256, None])
 @pytest.mark.parametrize("sinks,window", [(1, 1000), (64, 190), (65, 64), (130, 333), (190, 1)])
 @pytest.mark.parametrize("new", [7, 290])
