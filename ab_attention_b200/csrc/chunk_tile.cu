@@ -333,10 +333,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const ChunkArgs
                 }
                 u = chunk_unit(a, x, kGroups * kGroupRows, a.sorted != 0);
                 u.row0 += second * kGroupRows;
-                rows = u.seq < 0 ? 0 : min(most, u.n * a.group - u.row0);
+                rows = u.seq < 0 ? 0 : max(min(most, u.n * a.group - u.row0), 0);
                 n = begin = 0;
                 whole = false;
-                if (rows <= 0) return;
+                if (rows == 0) return;
                 // A lane for each row that matters: the tile's first and last, the groups' first and last.
                 const int which = lane < 2 ? (lane == 0 ? 0 : rows - 1)
                                            : (lane & 2 ? (lane & 1) * kGroupRows : min(((lane & 1) + 1) * kGroupRows, rows) - 1);
