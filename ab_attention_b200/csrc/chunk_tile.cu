@@ -15,8 +15,8 @@
 // group's other steps fill the other's. Bounds for a tile of both groups, in SM
 // cycles: tensor pipe 2,048 (four products of 128^3), exponential unit 2,048 (32,768 at
 // 16 a cycle), shared memory half as much again (operands 2,048, P 512, incoming K and V 512).
-// Measured for 3,600 rows x 12 heads over 75,600 keys (1,672 GFLOP): 1.43 ms alone
-// (1,170 TFLOP/s, tensor pipe and exponential unit 63% busy), 1.62 ms back to back,
+// Measured for 3,600 rows x 12 heads over 75,600 keys (1,672 GFLOP): 1.41 ms alone
+// (1,180 TFLOP/s, tensor pipe 61 and exponential unit 64% busy), 1.62 ms back to back,
 // where the GPU is at its power cap (993 W, 1.4 to 1.67 GHz) and fewer cycles no longer
 // shorten it.
 //
