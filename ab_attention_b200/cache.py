@@ -8,7 +8,7 @@ queries to everything stored, under a causal or block-causal rule with an option
 sliding window and sinks.
 
 Tokens are packed: q, k, v are [tokens, heads, 128], and sequence s owns tokens
-``starts[s]:starts[s + 1]``. ``lengths[s]`` counts its keys once the chunk is stored, so
+``starts[s]:starts[s + 1]`` (``starts`` never decreases). ``lengths[s]`` counts its keys once the chunk is stored, so
 token i of n sits at position ``lengths[s] - n + i``; position p lies in page
 ``page_table[s, p // page_size]``, row ``p % page_size``. All three are int32 on the
 device and are read there, so the calls never synchronise and can be captured into CUDA
@@ -68,9 +68,10 @@ def chunk_attention(q, cache, page_table, starts, lengths, *, longest=None, wind
 
     ``longest``: an upper bound of the tokens of any one sequence, known on the host (default:
     all tokens). Give it: a batch of short chunks takes another kernel than one long chunk. A
-    sequence with more tokens is not computed and sets the device error word.
-    Returns out [tokens, heads, 128] (rows behind the last sequence are left as they are in
-    ``out``, and undefined without it), and with ``return_lse`` the base-2 log-sum-exp
+    sequence with more tokens is not computed: its rows are left as they are and the device error
+    word is set.
+    Returns out [tokens, heads, 128] (rows behind the last sequence are left as they are too; both
+    kinds are undefined without ``out``), and with ``return_lse`` the base-2 log-sum-exp
     [tokens, heads] float32. Keys and values of a sequence have to be finite; rows of its last page
     behind its length are never used.
     """

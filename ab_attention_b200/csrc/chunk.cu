@@ -69,6 +69,24 @@ bool halves_end_sooner(const ChunkArgs& a, int jobs, int whole) {
     return with.end < without.end;
 }
 
+// Whether a call over ragged sequences computes packed token `token`: it lies in a sequence, and that has no more
+// tokens than the launch covers. The splits wrote nothing for any other row, so a join leaves it alone.
+__device__ __forceinline__ bool chunk_covers(const ChunkArgs& a, int64_t token) {
+    int lo = 0, hi = a.seqs;
+    if (token < __ldg(a.starts) || token >= __ldg(a.starts + hi)) return false;
+    while (hi - lo > 1) {  // starts[lo] <= token < starts[hi]
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(a.starts + mid) <= token)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    int32_t first, n, len;
+    bool bad;
+    chunk_sequence(a, lo, first, n, len, bad);
+    return token < first + n;
+}
+
 // Joins the splits of each row: o = sum_s 2^(lse_s - lse) o_s. A block a row, four dims a lane, each warp an
 // eighth of the splits; reads splits * 516 bytes a row.
 template <class T>
@@ -76,18 +94,20 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
     constexpr int kWarps = 8;
     __shared__ float4 part[kWarps][32];
     __shared__ float2 stat[kWarps];
-    cudaGridDependencySynchronize();
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t row = blockIdx.x;
     const int64_t token = row / a.heads;
     const int head = static_cast<int>(row - token * a.heads);
     int64_t seq = 0, at = token;
+    bool mine = true;
     if (a.starts == nullptr) {
         seq = token / a.tokens;
         at = token - seq * a.tokens;
-    } else if (token < __ldg(a.starts) || token >= __ldg(a.starts + a.seqs)) {
-        return;  // in no sequence: left as it was
+    } else {
+        mine = chunk_covers(a, token);  // else left as it was; read while the last splits still run
     }
+    cudaGridDependencySynchronize();
+    if (!mine) return;
     if (a.span > 0 && a.part_lse[row] == kWhole) return;  // written by its only split
     // This warp's splits w, w + 8, ..: 32 at a time, their sums' weights against a running maximum.
     float top = -INFINITY, sum = 0.f;
@@ -154,7 +174,6 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
 // a row's splits (eight at a time) go out together.
 template <class T>
 __global__ void __launch_bounds__(256) chunk_join_rows_kernel(const ChunkArgs a) {
-    cudaGridDependencySynchronize();
     const int lane = threadIdx.x & 7;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 3);
     const int64_t token = row / a.heads;
@@ -165,8 +184,9 @@ __global__ void __launch_bounds__(256) chunk_join_rows_kernel(const ChunkArgs a)
         seq = token / a.tokens;
         at = token - seq * a.tokens;
     } else {
-        mine = mine && token >= __ldg(a.starts) && token < __ldg(a.starts + a.seqs);  // else left as it was
+        mine = mine && chunk_covers(a, token);  // else left as it was; read while the last splits still run
     }
+    cudaGridDependencySynchronize();
     if (mine && a.span > 0) mine = a.part_lse[row] != kWhole;  // written by its only split
     const unsigned lanes = 0xffu << (threadIdx.x & 24);
     if (!mine) return;  // whole groups of eight lanes

@@ -282,8 +282,8 @@ int abx_rotary(const abx_rotary_args* args, abx_stream_t stream);
  * Paged: tokens are packed (`tokens` of all sequences; starts / lengths as above; the
  * sequence strides of q, o and lse are ignored), k and v are rows (page, head, token
  * of a page). page_size is 16, 32, 64 or a multiple of 128. longest bounds the tokens
- * of any sequence; a sequence with more is not computed and records
- * ABX_ERR_INVALID_ARGUMENT, as do lengths or starts past the buffers (clipped)
+ * of any sequence; a sequence with more is not computed (its rows are left as they
+ * were) and records ABX_ERR_INVALID_ARGUMENT, as do lengths or starts past the buffers (clipped)
  * and table entries that name no page (read as zeros). Rows of tokens in no
  * sequence are left as they were. The cached rows of a sequence have to be
  * finite; what lies behind them in its last page may be anything.
