@@ -123,7 +123,8 @@ class StreamAttention:
 
     Call the object once per layer and denoising step of a chunk (each call replaces the chunk's keys and
     values), then ``advance()`` once the chunk is final. Nothing synchronises: ``advance`` updates device
-    counters in place, so a captured step replays for chunk after chunk.
+    counters in place, so a captured step replays for chunk after chunk. Before a capture that has a layer's
+    first call, ``allocate(layers)`` makes the caches.
     """
 
     def __init__(self, heads, height, width, *, max_frames, kv_heads=None, chunk_frames=1, window_frames=None, sink_frames=0,
@@ -173,6 +174,15 @@ class StreamAttention:
         self.lengths.add_(self.tokens)
         self.positions[:, 0].add_(self.chunk_frames)
 
+    def allocate(self, layers):
+        """Creates the caches of these layers, where they have none. A layer's first call does it too, but not inside a
+        CUDA graph capture: memory and fill would be the graph's own, and every replay would clear the chunks before."""
+        missing = [layer for layer in layers if layer not in self.caches]
+        if missing and not self.page_table.is_cpu and torch.cuda.is_current_stream_capturing():
+            raise ValueError(f"layer {missing[0]!r} has no cache yet: call allocate(layers) before the capture")
+        for layer in missing:
+            self.caches[layer] = kv_cache(**self._cache)
+
     @torch.no_grad()
     def __call__(self, layer, q, k, v):
         """q [B,H,N,128], k and v [B,Hk,N,128] of the chunk's N tokens (before rotation), any strides with
@@ -181,8 +191,7 @@ class StreamAttention:
             raise ValueError(f"q must be {[self.batch, self.heads, self.tokens, 128]} (got {list(q.shape)})")
         if k.shape != (self.batch, self.kv_heads, self.tokens, 128) or v.shape != k.shape:
             raise ValueError(f"k and v must be {[self.batch, self.kv_heads, self.tokens, 128]}")
-        if layer not in self.caches:
-            self.caches[layer] = kv_cache(**self._cache)
+        self.allocate((layer,))
         cache, where = self.caches[layer], (self.page_table, self.starts, self.lengths)
         q, k, v = (x.transpose(1, 2).flatten(0, 1) for x in (q, k, v))  # packed; a view for one batch
         q = append_kv(cache, k, v, *where, positions=self.positions, axes=self.axes, q=q)

@@ -38,3 +38,45 @@ def test_rows_of_dropped_sequences_stay(sizes, longest, heads, kv):
             hold(out[rows], lse[rows], b.q[rows], b.k[s], b.v[s])
         at += m
     assert (out[at:] == 7).all() and (lse[at:] == 7).all()
+
+
+# ---- a stream whose first call is captured --------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("batch,window,sinks,frames", [(1, None, 0, 4), (2, 2, 1, 9)])
+def test_stream_attention_captured_first(batch, window, sinks, frames):
+    """A stream's first call of every layer may be in a capture once its caches are there; the replays give what
+    eager calls give. Without the caches the capture is refused."""
+    def stream():
+        return ab.StreamAttention(2, 5, 9, max_frames=frames, window_frames=window, sink_frames=sinks, batch=batch, page_size=16)
+
+    def inputs(f):
+        g = gen(f)
+        return [normal(g, batch, 2, 45, 128) for _ in range(3)]
+
+    eager, want = stream(), []
+    for f in range(frames):
+        q, k, v = inputs(f)
+        want.append([eager(layer, q, k + layer, v).clone() for layer in range(2)])
+        if f + 1 < frames:
+            eager.advance()
+    s, held = stream(), inputs(0)
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="allocate"), torch.cuda.graph(torch.cuda.CUDAGraph()):
+        s(0, *held)
+    s.allocate(range(2))
+    caches = dict(s.caches)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [s(layer, held[0], held[1] + layer, held[2]) for layer in range(2)]
+    for turn in range(2):
+        for f in range(frames):
+            for x, y in zip(held, inputs(f)):
+                x.copy_(y)
+            graph.replay()
+            for x, y in zip(outs, want[f]):
+                assert torch.equal(x, y)
+            if f + 1 < frames:
+                s.advance()
+        s.reset()
+    assert s.caches.keys() == caches.keys() and all(s.caches[x] is caches[x] for x in caches)
