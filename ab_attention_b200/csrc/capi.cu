@@ -732,7 +732,10 @@ int chunk_plan(const abx_chunk_args* c, abx::ChunkArgs& a, size_t& workspace) {
     const int64_t all_tokens = paged ? c->tokens : c->tokens * c->sequences;
     if (c->heads > 0x3fffffff || c->tokens > 0x3fffffff / c->heads || all_tokens > 0x7fffffff)
         return fail(ABX_ERR_UNSUPPORTED, "too many query rows");
-    const int64_t largest = 0x3fffffff;
+    // Positions stay below 2^30, so a block that is larger is one block over all of them; its window counts back
+    // from the block's end, and what of it lies past the largest block here hides no key.
+    const int64_t largest = 0x3fffffff, past = c->block > largest ? c->block - largest : 0;
+    const int64_t window = c->window > past ? c->window - past : 0;
     a = abx::ChunkArgs{};
     a.q = c->q;
     a.o = c->o;
@@ -756,7 +759,7 @@ int chunk_plan(const abx_chunk_args* c, abx::ChunkArgs& a, size_t& workspace) {
     for (int shift = 4; shift < 30; ++shift)
         if (a.page_size == 1 << shift) a.page_shift = shift;
     a.pages = static_cast<int32_t>(paged ? c->pages : c->sequences);
-    a.window = c->window == 0 ? abx::kNoWindow : static_cast<int32_t>(at_most(c->window, largest));
+    a.window = c->window == 0 ? abx::kNoWindow : static_cast<int32_t>(at_most(window, abx::kNoWindow - 1));
     a.sinks = c->window == 0 ? 0 : static_cast<int32_t>(at_most(c->sinks, largest));
     a.block = static_cast<int32_t>(at_most(c->block, largest));
     a.rows_total = all_tokens * c->heads;

@@ -53,7 +53,7 @@ struct ChunkArgs {
     int* error;
 };
 
-constexpr int32_t kNoWindow = 0x40000000;
+constexpr int32_t kNoWindow = 0x7fffffff;  // above every block's end
 constexpr int32_t kMaxCacheKeys = 0x3fffffff;
 constexpr int kMaxCluster = 8;
 constexpr int kChunkTokenKeys = 64;  // keys of a tile of each kernel

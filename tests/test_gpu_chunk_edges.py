@@ -1,5 +1,7 @@
 """Calls of the streaming operators at the edges of what their documentation allows, on the GPU. Tolerances
 as in test_gpu_chunk.py."""
+import math
+
 import pytest
 import torch
 
@@ -80,3 +82,39 @@ def test_stream_attention_captured_first(batch, window, sinks, frames):
                 s.advance()
         s.reset()
     assert s.caches.keys() == caches.keys() and all(s.caches[x] is caches[x] for x in caches)
+
+
+# ---- windows and blocks past 2^30 ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("window,block", [
+    (2 ** 40 - 5, 2 ** 40),      # the window of the only block ends five keys after the first
+    (2 ** 40 - 299, 2 ** 40),    # ... and after all but one
+    (2 ** 35, 2 ** 40),          # ... and past the last: only the sinks are seen
+    (2 ** 40, 2 ** 40), (2 ** 62, 2 ** 61), (2 ** 62, 2 ** 63 - 1), (2 ** 63 - 1, 1), (2 ** 30, 7), (2 ** 31, 2 ** 30 - 1),
+    (2 ** 30 + 3, 2 ** 30 + 5), (10, 2 ** 30), (None, 2 ** 63 - 1),
+])
+@pytest.mark.parametrize("tokens", [2, 300])
+def test_windows_and_blocks_of_any_size(window, block, tokens):
+    g, keys = gen(tokens), 300
+    q, k, v = normal(g, 1, 2, tokens, 128), normal(g, 1, 1, keys, 128), normal(g, 1, 1, keys, 128)
+    # the definition's own sizes stay within 64 bits: a block past all positions ends where it says
+    for sinks in (0, 3):
+        o, lse = ab.window_attention(q, k, v, window=window, sinks=sinks, block=block, return_lse=True)
+        hold(o[0].transpose(0, 1), lse[0].T, *(x[0].transpose(0, 1) for x in (q, k, v)), window=window, sinks=sinks, block=block)
+
+
+def test_block_that_ends_past_2_to_30():
+    """The second block of 805 million positions ends past 2^30, and without a window its tokens see all keys (of
+    one page, in every place of the table): equal scores of 0, so the base-2 log-sum-exp is that of their count."""
+    block, page = 0x30000000, 16384
+    keys = torch.zeros(1, 1, page, 128, dtype=torch.bfloat16, device="cuda")
+    values = torch.ones_like(keys)
+    width = block // page + 1
+    table = torch.zeros(1, width, dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([width * page], dtype=torch.int32, device="cuda")
+    q = torch.ones(1, 1, 128, dtype=torch.bfloat16, device="cuda")
+    o, lse = ab.chunk_attention(q, ab.KVCache(keys, values), table, starts, lengths, block=block, return_lse=True)
+    assert (o == 1).all()
+    assert abs(lse.item() - math.log2(width * page)) < 5e-4
