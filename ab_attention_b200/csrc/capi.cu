@@ -674,12 +674,21 @@ int check_pages(int64_t sequences, int64_t table_width, int64_t page_size, int64
     return ABX_OK;
 }
 
+// Whether a dim of more than one element repeats its rows by a stride of 0.
+bool repeats(const int64_t (&size)[3], const int64_t (&stride)[3]) {
+    for (int i = 0; i < 3; ++i)
+        if (size[i] > 1 && stride[i] == 0) return true;
+    return false;
+}
+
 // Four dims [128, d1, d2, d3] with strides in elements and 64 x b1 x b2 x 1 boxes, 128-byte swizzle. A
-// dim of one element may have any stride; the map wants one that it can encode.
+// dim of one element may have any stride; the map wants one that it can encode. Rows that repeat are refused: the
+// encoder takes a stride of 0, but nothing documents what a copy then does.
 cudaError_t encode_rows4d(CUtensorMap* map, const void* base, bool fp16, const int64_t (&size)[3], const int64_t (&stride)[3],
                           uint32_t b1, uint32_t b2) {
     auto encode = abx::tensor_map_encoder();
     if (encode == nullptr) return cudaErrorNotSupported;
+    if (repeats(size, stride)) return cudaErrorInvalidValue;
     cuuint64_t dims[4] = {abx::kHeadDim}, bytes[3];
     for (int i = 0; i < 3; ++i) {
         dims[i + 1] = static_cast<cuuint64_t>(size[i]);
@@ -729,6 +738,9 @@ int chunk_plan(const abx_chunk_args* c, abx::ChunkArgs& a, size_t& workspace) {
         if (c->keys > abx::kMaxCacheKeys || c->sequences > 0x3fffffff) return fail(ABX_ERR_UNSUPPORTED, "more than 2^30 keys");
         if (c->longest != c->tokens) return fail(ABX_ERR_INVALID_ARGUMENT, "longest must be the token count");
     }
+    const int64_t cache[3] = {paged ? c->pages : c->sequences, c->kv_heads, paged ? c->page_size : c->keys};
+    if (repeats(cache, c->k_stride) || repeats(cache, c->v_stride))
+        return fail(ABX_ERR_INVALID_ARGUMENT, "the rows of k and v must not repeat by a stride of 0");
     const int64_t all_tokens = paged ? c->tokens : c->tokens * c->sequences;
     if (c->heads > 0x3fffffff || c->tokens > 0x3fffffff / c->heads || all_tokens > 0x7fffffff)
         return fail(ABX_ERR_UNSUPPORTED, "too many query rows");

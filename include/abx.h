@@ -278,7 +278,8 @@ int abx_rotary(const abx_rotary_args* args, abx_stream_t stream);
  * h reads key head h / (heads / kv_heads).
  *
  * Contiguous (page_table NULL): q and o rows (sequence, head, token) of `tokens`
- * tokens a sequence, k and v rows (sequence, head, token) of `keys` tokens.
+ * tokens a sequence, k and v rows (sequence, head, token) of `keys` tokens. Rows of
+ * q may repeat (a stride of 0), those of k and v may not.
  * Paged: tokens are packed (`tokens` of all sequences; starts / lengths as above; the
  * sequence strides of q, o and lse are ignored), k and v are rows (page, head, token
  * of a page). page_size is 16, 32, 64 or a multiple of 128. longest bounds the tokens

@@ -118,3 +118,24 @@ def test_block_that_ends_past_2_to_30():
     o, lse = ab.chunk_attention(q, ab.KVCache(keys, values), table, starts, lengths, block=block, return_lse=True)
     assert (o == 1).all()
     assert abs(lse.item() - math.log2(width * page)) < 5e-4
+
+
+# ---- rows that repeat -----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim", [0, 1, 2])
+@pytest.mark.parametrize("heads,kv", [(4, 2), (6, 2)])
+def test_queries_that_repeat(heads, kv, dim):
+    """Batches, heads or tokens of many rows that repeat by a stride of 0: as contiguous queries."""
+    g = gen(dim)
+    q, k, v = normal(g, 2, heads, 900, 128), normal(g, 2, kv, 1500, 128), normal(g, 2, kv, 1500, 128)
+    one = q.narrow(dim, 0, 1).expand(2, heads, 900, 128)
+    for x, y in zip(ab.window_attention(one, k, v, window=700, return_lse=True),
+                    ab.window_attention(one.contiguous(), k, v, window=700, return_lse=True)):
+        assert torch.equal(x, y)
+    b = Batch(dim, [(700, 900), (300, 2000)], heads, kv, 32, torch.bfloat16)
+    if dim > 0:
+        one = b.q.narrow(2 - dim, 0, 1).expand(1000, heads, 128)
+        for x, y in zip(ab.chunk_attention(one, b.cache, *b.plan, longest=700, return_lse=True),
+                        ab.chunk_attention(one.contiguous(), b.cache, *b.plan, longest=700, return_lse=True)):
+            assert torch.equal(x, y)
