@@ -156,7 +156,8 @@ class StreamAttention:
         self.lengths = torch.empty(batch, dtype=torch.int32, device=device)
         self.positions = torch.empty(batch * self.tokens, 3, dtype=torch.int32, device=device)
         self._first = grid_positions(chunk_frames, height, width, device=device).repeat(batch, 1)
-        self._cache = dict(pages=places * batch, kv_heads=self.kv_heads, page_size=page_size, dtype=dtype, device=device)
+        self._cache = dict(pages=places * batch, kv_heads=self.kv_heads, page_size=page_size, dtype=dtype,
+                           device=self.page_table.device)  # with its index: the caches are made later
         self.caches = {}
         self.reset()
 
@@ -178,8 +179,10 @@ class StreamAttention:
         """Creates the caches of these layers, where they have none. A layer's first call does it too, but not inside a
         CUDA graph capture: memory and fill would be the graph's own, and every replay would clear the chunks before."""
         missing = [layer for layer in layers if layer not in self.caches]
-        if missing and not self.page_table.is_cpu and torch.cuda.is_current_stream_capturing():
-            raise ValueError(f"layer {missing[0]!r} has no cache yet: call allocate(layers) before the capture")
+        if missing and self.page_table.is_cuda:
+            with torch.cuda.device(self.page_table.device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise ValueError(f"layer {missing[0]!r} has no cache yet: call allocate(layers) before the capture")
         for layer in missing:
             self.caches[layer] = kv_cache(**self._cache)
 

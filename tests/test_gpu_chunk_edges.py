@@ -139,3 +139,16 @@ def test_queries_that_repeat(heads, kv, dim):
         for x, y in zip(ab.chunk_attention(one, b.cache, *b.plan, longest=700, return_lse=True),
                         ab.chunk_attention(one.contiguous(), b.cache, *b.plan, longest=700, return_lse=True)):
             assert torch.equal(x, y)
+
+
+# ---- another device -------------------------------------------------------------------------------------------------
+
+
+def test_stream_attention_keeps_its_device(monkeypatch):
+    """The caches of a stream are made on the device that it was made on, whichever is current at a layer's first call."""
+    made, kv_cache = [], ab.video.kv_cache
+    monkeypatch.setattr(ab.video, "kv_cache", lambda *, device, **more: made.append(device) or kv_cache(device=device, **more))
+    s = ab.StreamAttention(2, 5, 9, max_frames=2)
+    s.allocate("ab")
+    assert made == [s.page_table.device] * 2 and made[0].index is not None
+    assert all(x.device == s.page_table.device for cache in s.caches.values() for x in cache)
