@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import ab_attention_b200 as ab
+from oracle import stream
 from tests.test_gpu_chunk import Batch, clean_status, gen, hold, normal, reported  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -152,3 +153,24 @@ def test_stream_attention_keeps_its_device(monkeypatch):
     s.allocate("ab")
     assert made == [s.page_table.device] * 2 and made[0].index is not None
     assert all(x.device == s.page_table.device for cache in s.caches.values() for x in cache)
+
+
+# ---- fp16 over long rows ----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("tokens,keys,window,scale", [
+    (1, 60000, None, 1), (300, 20000, None, 1), (300, 9000, None, 4), (32, 40000, None, 4), (260, 30000, 8000, 1),
+])
+def test_fp16_keeps_small_weights(tokens, keys, window, scale):
+    """fp16 weights are lifted by 2^7 and the row's largest is at least its reference, so it is held as 2^7 or more.
+    A weight below fp16's normal range is off by 2^-25 at most, 2^-32 of the largest: keys * 2^-32 * max |v| in
+    all, beside what bf16 is held to with fp16's half step. Scores four times as large are off by four times as much."""
+    g, half = gen(keys), torch.float16
+    q = normal(g, 1, 4, tokens, 128, dtype=half) * scale
+    k, v = normal(g, 1, 2, keys, 128, dtype=half), normal(g, 1, 2, keys, 128, dtype=half)
+    o, lse = ab.window_attention(q, k, v, window=window, return_lse=True)
+    ref, ref_lse, a = stream.attend(*(x[0].transpose(0, 1) for x in (q, k, v)), window=window)
+    u = torch.finfo(half).eps / 2 * 1.01
+    tol = (u + 4e-4 * scale) * a + u * ref.abs() + 2 ** -25 + keys * 2 ** -32 * v.double().abs().max()
+    assert ((o[0].transpose(0, 1).double() - ref).abs() <= tol).all()
+    assert ((lse[0].T.double() - ref_lse).abs() <= 5e-4 * scale).all()
