@@ -269,7 +269,6 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
                         *reinterpret_cast<uint4*>(mem + st * kStage + kOperand +
                                                   chunk_at(warp * kWarpKeys + (x >> 4), x & 15, kSlab)) =
                             make_uint4(0, 0, 0, 0);
-                tc::fence_proxy_async_smem();  // before the next copy into this stage
                 __syncwarp();
             }
             // O += P V: V as [key][dim], transposed by the load; 16 dims a step.
@@ -285,6 +284,10 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
                     mma_16816<T>(o[x][2 * d + 1], rest[x], vb[2], vb[3]);
                 }
             }
+            // The next copy into this stage is another proxy's write: an arrival alone does not keep it behind the
+            // warp's reads (and clears). Without the fence, reads that waited behind other traffic of the SM, a storm
+            // of atomics say, found the tile three on.
+            tc::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(empty(st));
         }

@@ -174,3 +174,32 @@ def test_fp16_keeps_small_weights(tokens, keys, window, scale):
     tol = (u + 4e-4 * scale) * a + u * ref.abs() + 2 ** -25 + keys * 2 ** -32 * v.double().abs().max()
     assert ((o[0].transpose(0, 1).double() - ref).abs() <= tol).all()
     assert ((lse[0].T.double() - ref_lse).abs() <= 5e-4 * scale).all()
+
+
+# ---- the few-row kernel's ring of tiles under other traffic ---------------------------------------------------------
+
+
+@pytest.mark.parametrize("page", [16, 128])
+def test_tiles_stay_until_they_are_read(page):
+    """Every CTA reports the sequences that are too long, which keeps the SMs' memory paths busy with atomics while
+    the others' tiles are read: no tile may be written over before that. Equal calls give equal rows."""
+    sizes = [(2, 357), (8, 74), (8, 407), (7, 1817), (8, 303), (1, 1979), (1, 1314), (1, 1456), (4, 1297), (1, 2307)] * 2
+    sizes += [(8, 1591 - 40 * i) for i in range(14)] + [(1, 1528), (3, 1661), (1, 2172), (1, 2023), (2, 395), (1, 971)]
+    b = Batch(page, sizes, 8, 8, page, torch.bfloat16)
+    rows, at = [], 0
+    for m, _ in sizes:
+        rows += range(at, at + m) if m <= 3 else []
+        at += m
+    first = None
+    for turn in range(60):
+        o, lse = ab.chunk_attention(b.q, b.cache, *b.plan, longest=3, return_lse=True)
+        o, lse = o[rows], lse[rows]
+        if first is None:
+            first, at = (o, lse), 0
+            for s, (m, n) in enumerate(sizes):
+                if m <= 3:
+                    q = b.q[sum(x for x, _ in sizes[:s]):][:m]
+                    hold(o[at:at + m], lse[at:at + m], q, b.k[s], b.v[s])
+                    at += m
+        assert torch.equal(o, first[0]) and torch.equal(lse, first[1])
+    assert reported() == 1
