@@ -67,7 +67,9 @@ def chunk_attention(q, cache, page_table, starts, lengths, *, longest=None, wind
     ``h // (heads // kv_heads)``.
 
     ``longest``: an upper bound of the tokens of any one sequence, known on the host (default:
-    all tokens). Give it: a batch of short chunks takes another kernel than one long chunk. A
+    all tokens). Give it: a batch of short chunks takes another kernel than one long chunk. The other
+    bound that a call is planned by is the table's width (the lengths are on the device): a table much wider
+    than the longest sequence gives the same results, and a few short sequences take up to 2.4 times as long. A
     sequence with more tokens is not computed: its rows are left as they are and the device error
     word is set.
     Returns out [tokens, heads, 128] (rows behind the last sequence are left as they are too; both

@@ -14,11 +14,13 @@
 // rate and the unit idled through the rest of the tile (3,850 cycles); in turns one
 // group's other steps fill the other's. Bounds for a tile of both groups, in SM
 // cycles: tensor pipe 2,048 (four products of 128^3), exponential unit 2,048 (32,768 at
-// 16 a cycle), shared memory half as much again (operands 2,048, P 512, incoming K and V 512).
-// Measured for 3,600 rows x 12 heads over 75,600 keys (1,672 GFLOP): 1.41 ms alone
-// (1,180 TFLOP/s, tensor pipe 61 and exponential unit 64% busy), 1.62 ms back to back,
-// where the GPU is at its power cap (993 W, 1.4 to 1.67 GHz) and fewer cycles no longer
-// shorten it.
+// 16 a cycle), shared memory half as much again (3,072: operands 2,048, P 512, incoming K and V
+// 512), and that is what a step of 3,130 cycles is bound by.
+// Measured for 3,600 rows x 12 heads over 75,600 keys (1,672 GFLOP): 1.41 to 1.45 ms alone
+// (1,180 TFLOP/s, tensor pipe 61 and exponential unit 64% busy), 1.62 ms back to back, where the
+// power cap (980 W) takes the clock to 1.58 GHz; cuDNN's attention on the same call: 1.78 and 1.81 ms.
+// Cycles still count under the cap: over 75,520 rows cuDNN has 1,356 TFLOP/s at 1.43 GHz,
+// this kernel 1,168 at 1.55.
 //
 // CTAs are persistent: near the end of its rows a CTA asks the grid's launch control for
 // the place of a CTA that has not started and goes on with that. Set-up and hand-over

@@ -13,7 +13,7 @@
 // With few sequences the keys are split over CTAs as well, joined in a cluster (up to
 // eight) or by a second kernel. One token of 12 heads over 131,001 keys in pages
 // of 16: 131 us (6.1 TB/s, 94% of the copy rate); 48 ragged sequences, 32 heads on 8:
-// 263 us (6.0 TB/s).
+// 268 us (5.9 TB/s).
 #include <type_traits>
 
 #include "chunk.cuh"
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kThreads) chunk_token_kernel(const ChunkArgs a
 #pragma unroll
             for (int x = 0; x < MT; ++x) {
                 // The maximum is kept as the bare score: s - m is exact where it matters, so the
-                // largest weight of a row is 1 (or 2^8 at most) however large the scores are.
+                // largest weight of a row is 1 (or 2^8 at most) however large the scores are, times 2^kLift.
                 float top[2];
                 bool grow = false;
 #pragma unroll

@@ -49,7 +49,7 @@ def _on_gpu(x: torch.Tensor) -> None:
 def apply_rotary(q, k, positions, axes=VIDEO_AXES, *, inverse=False):
     """Turns q [B, H, N, 128] and k [B, Hk, N, 128] (or None); bf16, fp16 or f32.
 
-    positions: int32 [N, axes] or [B, N, axes]. Returns contiguous (q, k). Rows may be
+    positions: int32 [N, axes] or [B, N, axes]. Returns contiguous (q, k), which carry no gradient. Rows may be
     strided (a [B, N, H, 128] projection transposed to [B, H, N, 128]) as long as the 128
     dims are contiguous and rows start on 16-byte boundaries; else they are copied first.
     """

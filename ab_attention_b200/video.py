@@ -189,14 +189,15 @@ class StreamAttention:
     @torch.no_grad()
     def __call__(self, layer, q, k, v):
         """q [B,H,N,128], k and v [B,Hk,N,128] of the chunk's N tokens (before rotation), any strides with
-        contiguous rows; returns [B,H,N,128], a view of token-major [B,N,H,128] memory."""
+        contiguous rows; returns [B,H,N,128], a view of token-major [B,N,H,128] memory. A batch of more than one is
+        copied first unless q, k and v are such views too (projections as they come, transposed)."""
         if q.shape != (self.batch, self.heads, self.tokens, 128):
             raise ValueError(f"q must be {[self.batch, self.heads, self.tokens, 128]} (got {list(q.shape)})")
         if k.shape != (self.batch, self.kv_heads, self.tokens, 128) or v.shape != k.shape:
             raise ValueError(f"k and v must be {[self.batch, self.kv_heads, self.tokens, 128]}")
         self.allocate((layer,))
         cache, where = self.caches[layer], (self.page_table, self.starts, self.lengths)
-        q, k, v = (x.transpose(1, 2).flatten(0, 1) for x in (q, k, v))  # packed; a view for one batch
+        q, k, v = (x.transpose(1, 2).flatten(0, 1) for x in (q, k, v))  # packed; a view for one batch, or of token-major memory
         q = append_kv(cache, k, v, *where, positions=self.positions, axes=self.axes, q=q)
         out = chunk_attention(q, cache, *where, longest=self.tokens, window=self.window, sinks=self.sinks, block=self.tokens)
         return out.unflatten(0, (self.batch, self.tokens)).transpose(1, 2)

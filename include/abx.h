@@ -249,7 +249,7 @@ enum abx_dtype { ABX_BF16 = 0, ABX_FP16 = 1, ABX_F32 = 2 };
  * NULL: k is stored as it is (and q must be NULL). A token outside every
  * sequence is not stored; one whose place is outside the table, or whose table
  * entry names no page, is not stored and records ABX_ERR_INVALID_ARGUMENT in the
- * device error word. Two tokens with one place leave either's row. */
+ * device error word. Two tokens with one place leave parts of either's row. */
 typedef struct abx_rotary_args {
   int32_t dtype;
   int32_t axes;
